@@ -222,12 +222,116 @@ FA2_API int fa2_bwd_static(const fa2_bwd_args* args, void* stream);
  * library image and allocates nothing. No counterpart in the reference crate. */
 FA2_API int fa2_bwd_static_status(int device);
 
+/* ---------------------------------------------------------------------------------------------------------------
+ * Operators on a paged K/V cache: rotary positions, append, attention of the newest tokens, eviction. Every struct starts
+ * with its own size. The reference's counterparts of the cache (append with rotary, paged decoding) are
+ * flash-attn2-rs/src/host/cache/mod.rs:321,382 and src/device/varlen/paged.rs:26-299; positions with several axes and the
+ * eviction have none. */
+
+/* A pool of pages k, v [num_pages, page_size, heads_k, head_dim] with any outer strides {page, row, head} (in elements,
+ * multiples of 8; 16-byte aligned bases), and who has which pages. Token t of sequence b lies in row t % page_size of page
+ * block_table[b][t / page_size]. Two sequences may have pages in common where nothing writes to them. Entries are checked on
+ * the device: a page outside the pool is neither read nor written, its keys are seen by no row, and fa2_device_status() says
+ * 100; where a length exceeds what the table has room for (or max_seqlen_k) it is cut, and the status is 101. */
+typedef struct fa2_paged_cache {
+  int64_t size; /* sizeof(fa2_paged_cache) */
+  void* k;
+  void* v;
+  int64_t k_stride[3], v_stride[3];
+  float* attn_mass;           /* contiguous fp32 [num_pages, heads_k, page_size], or NULL: weight that each key has got */
+  const int32_t* block_table; /* device int32 [batch, max_pages], unit stride in a row; entries that no token needs are ignored */
+  int64_t block_table_stride;
+  const int32_t* seqlens_k;   /* device int32 [batch]: tokens in the cache */
+  int32_t num_pages, page_size, max_pages, batch, heads_k, head_dim, dtype;
+  int32_t reserved;           /* 0 */
+} fa2_paged_cache;
+
+/* Rotary positions with several axes (time, height, width, ...). The first 2 * (sections[0] + ... ) elements of a head are
+ * pairs: elements i and i + n of n pairs, or with interleaved_pairs elements 2 i and 2 i + 1; the rest is copied. A pair is
+ * turned by position[axis] * inv_freq[pair], worked out so that it is exact to a few 1e-7 rad at any position below 2^31.
+ * Which axis: the first sections[0] pairs have axis 0, the next sections[1] axis 1 and so on; with interleaved_axes pair i has
+ * axis i % axes while i < axes * sections[i % axes], and axis 0 behind that. inverse = 1 turns back: the gradient. */
+typedef struct fa2_rotary_args {
+  int64_t size; /* sizeof(fa2_rotary_args) */
+  const void* q; /* [batch, seqlen, heads, head_dim], or NULL */
+  void* q_out;
+  const void* k; /* [batch, seqlen, heads_k, head_dim], or NULL */
+  void* k_out;   /* ignored by fa2_paged_append */
+  int64_t q_stride[3], q_out_stride[3], k_stride[3], k_out_stride[3]; /* {batch, row, head}, any; the last stride is 1 */
+  const void* positions;  /* device [axes, batch, seqlen], int32 or int64 */
+  int64_t position_stride[3]; /* {axis, batch, row} */
+  const float* inv_freq;  /* device fp32, one per pair */
+  int32_t position_bits;  /* 32 or 64 */
+  int32_t dtype;
+  int32_t batch, seqlen, heads, heads_k, head_dim;
+  int32_t axes;           /* 1..4 */
+  int32_t sections[4];
+  int32_t interleaved_axes, interleaved_pairs, inverse;
+  int32_t reserved;       /* 0 */
+} fa2_rotary_args;
+FA2_API int fa2_rotary(const fa2_rotary_args* args, void* stream);
+
+/* New tokens: turn->q is turned into turn->q_out, turn->k into the cache behind the seqlens_k tokens that each sequence has
+ * there, and v is copied beside it; seqlens_k stays as it is. Dense: row i of sequence b is its new token i, and with
+ * seqlens_new only the first seqlens_new[b] rows are. Packed (cu_seqlens; turn->batch is 1): the new tokens of sequence b are
+ * the rows [cu_seqlens[b], cu_seqlens[b + 1]). Other rows are not written to the cache; every row of q is turned. */
+typedef struct fa2_paged_append_args {
+  int64_t size; /* sizeof(fa2_paged_append_args) */
+  const fa2_rotary_args* turn;
+  const fa2_paged_cache* cache;
+  const void* v;
+  int64_t v_stride[3];
+  const int32_t* cu_seqlens;  /* device int32 [cache->batch + 1], or NULL */
+  const int32_t* seqlens_new; /* device int32 [cache->batch], or NULL */
+} fa2_paged_append_args;
+FA2_API int fa2_paged_append(const fa2_paged_append_args* args, void* stream);
+
+/* Attention of the last seqlen_q tokens of every sequence (which the cache holds already) over its pages: token i of them sees
+ * the keys up to itself, with window_left >= 0 no more than window_left before it. At most 128 query rows per kv head
+ * (seqlen_q * heads / heads_k). A row without keys gives O = 0 and LSE = +inf. With cache->attn_mass the weights of each key,
+ * summed over the query rows of its kv head, are added to it. The workspace is 256-byte aligned and may hold anything;
+ * fa2_paged_fwd_workspace_bytes() bytes of it are needed (it grows with max_seqlen_k where there is attn_mass). A call
+ * repeats itself bit for bit, attn_mass of pages that sequences share excepted. */
+typedef struct fa2_paged_fwd_args {
+  int64_t size; /* sizeof(fa2_paged_fwd_args) */
+  const fa2_paged_cache* cache;
+  const void* q; /* [batch, seqlen_q, heads, head_dim] */
+  void* out;
+  float* lse;    /* contiguous fp32 [batch, heads, seqlen_q] */
+  int64_t q_stride[3], o_stride[3];
+  int32_t seqlen_q, heads;
+  float softmax_scale;
+  int32_t window_left; /* < 0 = unbounded */
+  float softcap;       /* 0 = off */
+  int32_t max_seqlen_k; /* bound on seqlens_k, or 0: what the table has room for */
+} fa2_paged_fwd_args;
+FA2_API int64_t fa2_paged_fwd_workspace_bytes(const fa2_paged_fwd_args* args);
+FA2_API int fa2_paged_fwd(const fa2_paged_fwd_args* args, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Eviction. Of a sequence with more than `budget` tokens every kv head keeps its newest `recent` tokens and, of the others, the
+ * budget - recent with the largest attn_mass (of equal ones the earlier; NaN counts as the largest). Shorter sequences keep
+ * all. The rows that are kept, with their attn_mass, go in their order to the pages of dst_block_table; the old pages stay as
+ * they are. No page of dst_block_table may be one that block_table names, or be named twice. seqlens_out[b] is the new
+ * length, kept[b][head] lists the old places of the rows, -1 behind the last. */
+typedef struct fa2_paged_evict_args {
+  int64_t size; /* sizeof(fa2_paged_evict_args) */
+  const fa2_paged_cache* cache; /* with attn_mass */
+  const int32_t* dst_block_table; /* device int32 [batch, dst_max_pages] */
+  int64_t dst_block_table_stride;
+  int32_t dst_max_pages, budget, recent;
+  int32_t reserved; /* 0 */
+  int32_t* seqlens_out; /* [batch] */
+  int32_t* kept;        /* [batch, heads_k, budget] */
+} fa2_paged_evict_args;
+FA2_API int fa2_paged_evict(const fa2_paged_evict_args* args, void* stream);
+
 /* Message of the last failed call on this thread ("" if none). */
 FA2_API const char* fa2_last_error(void);
 
 /* Synchronises `device` and returns the kernels' status word: 0 = every pipeline wait
  * completed; otherwise the code of the first wait that ran out (the kernels bound every
- * wait instead of spinning forever). Clears the word. Negative on CUDA failure. */
+ * wait instead of spinning forever), 100 or 101 = a call on a paged cache met a page or a length that cannot be. Clears the
+ * word. Negative on CUDA failure. */
 FA2_API int fa2_device_status(int device);
 
 /* Number of SMs the persistent kernels size their grids for on `device`. */

@@ -3,6 +3,7 @@
   lib/libfa2_b200.so            CUDA kernels + the C ABI declared in include/fa2_b200.h
   lib/libflash_attn2_b200.so    tvm-ffi operator symbols (__tvm_ffi_fwd, ...) on top of the C ABI
   lib/_fa2_torch.so             Python module: the dense calls on torch tensors, on top of the C ABI
+  lib/_fa2_paged.so             Python module: the operators on a paged K/V cache, the same way
 
 Run as `python build.py` or call build(); a library is rebuilt only when a source is newer.
 """
@@ -26,7 +27,8 @@ NVCC_FLAGS = [
     "-Xcompiler", "-fPIC,-fvisibility=hidden",
 ]
 
-KERNEL_SOURCES = ["fwd_sm100.cu", "fwd_wide_sm100.cu", "fwd_decode_sm100.cu", "bwd_sm100.cu", "bwd_pair_sm100.cu", "bwd_dq_sm100.cu", "bwd_wide_sm100.cu", "bwd_wide_pair_sm100.cu", "bwd_aux.cu", "fa2_host.cu"]
+KERNEL_SOURCES = ["fwd_sm100.cu", "fwd_wide_sm100.cu", "fwd_decode_sm100.cu", "bwd_sm100.cu", "bwd_pair_sm100.cu", "bwd_dq_sm100.cu", "bwd_wide_sm100.cu", "bwd_wide_pair_sm100.cu", "bwd_aux.cu", "fa2_host.cu",
+                  "rotary_sm100.cu", "fwd_paged_sm100.cu", "paged_evict_sm100.cu", "fa2_paged_host.cu"]
 
 
 def _newer(target: Path, deps: list[Path]) -> bool:
@@ -89,14 +91,14 @@ def build_tvm_ffi() -> Path | None:
     return out
 
 
-def build_torch_calls() -> Path:
+def build_torch_calls(source: str, module: str) -> Path:
     import sysconfig
 
     import torch
     from torch.utils.cpp_extension import include_paths
 
-    src = CSRC / "torch_calls.cc"
-    out = LIB / "_fa2_torch.so"
+    src = CSRC / source
+    out = LIB / f"{module}.so"
     if _newer(out, [src, INCLUDE / "fa2_b200.h", LIB / "libfa2_b200.so"]):
         libdir = Path(torch.__file__).resolve().parent / "lib"
         incs = [*include_paths(), sysconfig.get_paths()["include"], "/usr/local/cuda/include"]
@@ -111,7 +113,8 @@ def build_torch_calls() -> Path:
 def build(verbose: bool = False) -> None:
     build_kernels(verbose)
     build_tvm_ffi()
-    build_torch_calls()
+    build_torch_calls("torch_calls.cc", "_fa2_torch")
+    build_torch_calls("paged_calls.cc", "_fa2_paged")
 
 
 if __name__ == "__main__":

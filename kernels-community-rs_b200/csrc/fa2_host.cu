@@ -5,6 +5,7 @@
 #include "../../include/fa2_b200.h"
 #include "fa2_launch.h"
 #include "fa2_plan.h"
+#include "fa2_runtime.h"
 
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -20,6 +21,12 @@
 namespace {
 
 using fa2::BwdSplit;
+using fa2::DeviceScope;
+using fa2::fail;
+using fa2::g_error;
+using fa2::get_runtime;
+using fa2::kMaxDevices;
+using fa2::Runtime;
 using fa2::bwd_takes_pairs;
 using fa2::bwd_wide_takes_pairs;
 using fa2::DecodePlan;
@@ -32,6 +39,19 @@ using fa2::Scratch;
 using fa2::StreamPlan;
 using fa2::Windows;
 
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+constexpr int kStatusWords = 16;
+Runtime g_rt[kMaxDevices];
+std::mutex g_mu;
+EncodeTiledFn g_encode = nullptr;
+
+}  // namespace
+
+namespace fa2 {
+
 thread_local char g_error[512] = "";
 
 int fail(int code, const char* fmt, ...) {
@@ -41,24 +61,6 @@ int fail(int code, const char* fmt, ...) {
   va_end(ap);
   return code;
 }
-
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-// Per-device state, created on first use (the reference keeps the same kind of lazily built,
-// never-freed per-device runtime: flash-attn2-rs/src/host/runtime.rs:68-84).
-struct Runtime {
-  bool ready = false;
-  int sm_count = 0;
-  int cc_major = 0;
-  int* status = nullptr;  // device status word
-};
-constexpr int kMaxDevices = 64;
-constexpr int kStatusWords = 16;
-Runtime g_rt[kMaxDevices];
-std::mutex g_mu;
-EncodeTiledFn g_encode = nullptr;
 
 int get_runtime(int device, Runtime** out) {
   if (device < 0 || device >= kMaxDevices) return fail(FA2_E_VALUE, "device index %d out of range", device);
@@ -92,6 +94,27 @@ int get_runtime(int device, Runtime** out) {
   *out = &rt;
   return FA2_OK;
 }
+
+DeviceScope::DeviceScope(const void* ptr) {
+  cudaGetDevice(&prev_);
+  device_ = prev_;
+  cudaPointerAttributes attr;
+  if (ptr != nullptr && cudaPointerGetAttributes(&attr, ptr) == cudaSuccess &&
+      (attr.type == cudaMemoryTypeDevice || attr.type == cudaMemoryTypeManaged) && attr.device >= 0)
+    device_ = attr.device;
+  else
+    cudaGetLastError();  // an unknown pointer is not an error of this call
+  // Also when it is current already: a thread that has made no runtime call yet (autograd's) has no context bound,
+  // and the driver's tensor-map encoder needs one.
+  cudaSetDevice(device_);
+}
+DeviceScope::~DeviceScope() {
+  if (device_ != prev_) cudaSetDevice(prev_);
+}
+
+}  // namespace fa2
+
+namespace {
 
 // 4-D map over [batch][rows][heads][D] with arbitrary (16-byte multiple) outer strides; the
 // box is one 128-byte swizzle line wide and `box_rows` rows tall.
@@ -147,36 +170,6 @@ int check_layout(const void* ptr, const int64_t* stride, int nstride, const char
       return fail(FA2_E_VALUE, "%s: outer strides must be non-negative multiples of 8 elements", name);
   return FA2_OK;
 }
-
-// Makes the device that owns `ptr` current for the lifetime of the object and restores the caller's
-// device afterwards, as the reference binds the context of q before every launch
-// (flash-attn2-rs/src/host/forward/mod.rs:716-718). A pointer the runtime does not know (or a null
-// one) leaves the current device as it is.
-class DeviceScope {
- public:
-  explicit DeviceScope(const void* ptr) {
-    cudaGetDevice(&prev_);
-    device_ = prev_;
-    cudaPointerAttributes attr;
-    if (ptr != nullptr && cudaPointerGetAttributes(&attr, ptr) == cudaSuccess &&
-        (attr.type == cudaMemoryTypeDevice || attr.type == cudaMemoryTypeManaged) && attr.device >= 0)
-      device_ = attr.device;
-    else
-      cudaGetLastError();  // an unknown pointer is not an error of this call
-    // Also when it is current already: a thread that has made no runtime call yet (autograd's) has no context bound,
-    // and the driver's tensor-map encoder needs one.
-    cudaSetDevice(device_);
-  }
-  ~DeviceScope() {
-    if (device_ != prev_) cudaSetDevice(prev_);
-  }
-  DeviceScope(const DeviceScope&) = delete;
-  DeviceScope& operator=(const DeviceScope&) = delete;
-  int device() const { return device_; }
-
- private:
-  int prev_ = 0, device_ = 0;
-};
 
 __global__ void fill_empty_kernel(uint16_t* out, float* lse, int64_t rows, int heads, int d, int64_t o_row_stride,
                                   int64_t o_head_stride, int64_t o_batch_stride, int64_t rows_per_batch,

@@ -1,0 +1,95 @@
+// Kernel-side parameter blocks of the operators on a paged K/V cache.
+#pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "paged_index.h"
+
+namespace fa2 {
+
+// Codes of the status word besides WaitSite's.
+enum PagedFault : int {
+  kPagedBadPage = 100,   // an entry of a block table names no page of the pool, or a token lies past the table's row
+  kPagedTooLong = 101,   // a length exceeds the table's row, or the bound that the caller gave
+};
+
+// Strides of a tensor in elements: {batch (or page), row, head}.
+struct Strides3 {
+  int64_t outer, row, head;
+};
+
+// Rotary positions: q -> q_out, k -> k_out. With `append` k_out and v_out are the pools of the cache.
+struct RotaryParams {
+  const void *q, *k, *v;        // null: not there
+  void *q_out, *k_out, *v_out;
+  Strides3 qs, ks, vs, qos, kos, vos;
+  int tokens;                   // batch * seqlen
+  FastDiv seqlen, heads_all, items;  // rows per batch entry; heads of q, k (and v); 16-element items of a head
+  int heads, heads_k, head_dim, pairs;
+  int tokens_per_block;
+  const void* positions;
+  int64_t pos_axis, pos_batch, pos_row;
+  int positions64;
+  const float* inv_freq;
+  int axes, in_turns, neighbours, negate;  // neighbours: a pair is two neighbouring elements
+  int32_t sections[kMaxAxes];
+  // append
+  PageTable table;
+  const int32_t* seqlens;       // tokens already in the cache
+  const int32_t* cu_seqlens;    // packed: the tokens of sequence b are [cu[b], cu[b + 1])
+  const int32_t* seqlens_new;   // dense: only the first of each sequence's rows are tokens
+  int sequences;
+  int* status;
+};
+
+// Attention of the newest tokens over a paged cache (fwd_paged_sm100.cu).
+struct PagedParams {
+  const void *q, *k, *v;
+  void* o;
+  float* lse;                   // [batch, heads, seqlen_q]
+  Strides3 qs, ks, vs, os;
+  PageTable table;
+  const int32_t* seqlens;
+  int most_keys;                // longer sequences are cut to it
+  int batch, heads, heads_k, seqlen_q, head_dim;
+  FastDiv group;                // heads / heads_k
+  int rows, row_tiles;          // seqlen_q * group, in tiles of 16
+  int window;
+  float scale, scale_log2, softcap;
+  float* partials;              // 2 slots per CTA
+  unsigned long long* flags;    // one per slot: launch_tag once the part is in memory
+  unsigned long long launch_tag;
+  float* scores;                // [batch, heads_k, rows, score_stride] in the log2 domain, or null
+  int64_t score_stride;
+  float2* stats;                // [batch, heads_k, rows]: row maximum (log2 domain), 1 / row sum
+  float* mass;                  // [pages, heads_k, page_size]
+  int* status;
+};
+
+// Eviction (paged_evict_sm100.cu).
+struct EvictParams {
+  void *k, *v;
+  float* mass;
+  Strides3 ks, vs;
+  PageTable from, to;
+  const int32_t* seqlens;
+  int32_t* seqlens_out;
+  int32_t* kept;                // [batch, heads_k, budget]
+  int batch, heads_k, head_dim, budget, recent;
+  int* status;
+};
+
+cudaError_t launch_rotary(const RotaryParams& p, bool bf16, bool append, bool vectors, cudaStream_t stream);
+
+constexpr int kPagedRows = 16;       // query rows of a unit
+constexpr int kPagedMaxRows = 128;   // query rows per kv head
+// Keys that a CTA takes at a time.
+inline int paged_tile_keys(int head_dim) { return head_dim > 128 ? 64 : 128; }
+// Floats of a partial result: O of 16 rows, their maxima and sums.
+inline int64_t paged_part_floats(int head_dim) { return kPagedRows * (static_cast<int64_t>((head_dim + 63) / 64 * 64) + 2); }
+cudaError_t launch_fwd_paged(const PagedParams& p, int grid, bool bf16, cudaStream_t stream);
+cudaError_t launch_paged_mass(const PagedParams& p, int sm_count, cudaStream_t stream);
+
+cudaError_t launch_paged_evict(const EvictParams& p, int sm_count, cudaStream_t stream);
+
+}  // namespace fa2

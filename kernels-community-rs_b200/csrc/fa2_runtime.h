@@ -1,0 +1,39 @@
+// What the host files of the C ABI share: the error message, the state of a device, and the scope of a call's device.
+#pragma once
+
+namespace fa2 {
+
+// Message of the last failed call on this thread.
+extern thread_local char g_error[512];
+// Keeps the message, returns the code.
+int fail(int code, const char* fmt, ...);
+
+constexpr int kMaxDevices = 64;
+
+// Per-device state, created on first use (the reference keeps the same kind of lazily built,
+// never-freed per-device runtime: flash-attn2-rs/src/host/runtime.rs:68-84).
+struct Runtime {
+  bool ready = false;
+  int sm_count = 0;
+  int cc_major = 0;
+  int* status = nullptr;  // device status word
+};
+int get_runtime(int device, Runtime** out);
+
+// Makes the device that owns `ptr` current for the lifetime of the object and restores the caller's
+// device afterwards, as the reference binds the context of q before every launch
+// (flash-attn2-rs/src/host/forward/mod.rs:716-718). A pointer the runtime does not know (or a null
+// one) leaves the current device as it is.
+class DeviceScope {
+ public:
+  explicit DeviceScope(const void* ptr);
+  ~DeviceScope();
+  DeviceScope(const DeviceScope&) = delete;
+  DeviceScope& operator=(const DeviceScope&) = delete;
+  int device() const { return device_; }
+
+ private:
+  int prev_ = 0, device_ = 0;
+};
+
+}  // namespace fa2

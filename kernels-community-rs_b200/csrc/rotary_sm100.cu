@@ -1,0 +1,273 @@
+// Rotary positions with several axes for sm_100a (B200), alone and with the append of new tokens to a paged cache.
+//
+//   y0 = x0 cos a - x1 sin a,  y1 = x1 cos a + x0 sin a,   a = position[axis(pair)] * inv_freq[pair]
+//
+// for the pairs (x0, x1) of a head's first elements; the others are copied. The gradient is the turn by -a.
+//
+// What bounds it: 4 bytes of memory traffic an element. The angles of a token serve all of its heads, so a block takes a few
+// tokens whole: it starts the loads of its first elements, works out the cosines and sines of its tokens into shared memory
+// meanwhile, and then streams the heads through, 16 elements a thread. (A table of cosines and sines in memory would add 8
+// bytes a pair and a lookup; here a pair costs one sincos for 20 to 40 heads.)
+//
+// Angles: a position of 2^20 times a frequency of 1 in 32 bits is off by 0.03 to 0.06 rad. The frequency goes, by way of fp64,
+// into turns as a fixed-point fraction of 64 bits; times the position, modulo 2^64, that is the angle's fraction of a turn, off by
+// at most position * 2^-53 * (frequency's turns) + 2^-64 * position. What is left to round is that fraction to 24 bits.
+#include "sm100_ptx.cuh"
+#include "fa2_launch.h"
+#include "fa2_paged_params.h"
+
+namespace fa2 {
+
+namespace {
+
+constexpr int kThreads = 256;
+
+// cos and sin of position * frequency.
+__device__ __forceinline__ float2 turn_of(int64_t position, float frequency) {
+  double t = static_cast<double>(frequency) * 0.15915494309189533577;  // 1 / (2 pi)
+  t -= floor(t);
+  const uint64_t u = __double2ull_rn(t * 18446744073709551616.0);
+  const int64_t fraction = static_cast<int64_t>(u * static_cast<uint64_t>(position));  // [-1/2, 1/2) turns
+  float s, c;
+  sincospif(static_cast<float>(fraction) * 0x1p-63f, &s, &c);
+  if (!isfinite(frequency)) s = c = __int_as_float(0x7fffffff);
+  return make_float2(c, s);
+}
+
+__device__ __forceinline__ float2 turn_of_pair(const RotaryParams& p, int b, int s, int pair) {
+  const int axis = axis_of_pair(pair, p.axes, p.sections, p.in_turns != 0);
+  const int64_t at = axis * p.pos_axis + b * p.pos_batch + s * p.pos_row;
+  const int64_t position = p.positions64 ? static_cast<const int64_t*>(p.positions)[at] : static_cast<const int32_t*>(p.positions)[at];
+  float2 cs = turn_of(position, p.inv_freq[pair]);
+  if (p.negate) cs.y = -cs.y;
+  return cs;
+}
+
+// Where a new token goes: element offsets of its row (head 0) in the pools, or -1 where it is not written.
+__device__ __forceinline__ longlong2 cache_row(const RotaryParams& p, int token, int b, int s) {
+  int sequence = b, i = s;
+  if (p.cu_seqlens != nullptr) {
+    // the last sequence that begins at or before the token
+    int lo = 0, hi = p.sequences;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (p.cu_seqlens[mid] <= token) lo = mid + 1;
+      else hi = mid;
+    }
+    sequence = lo - 1;
+    if (sequence < 0 || token >= p.cu_seqlens[sequence + 1]) return make_longlong2(-1, -1);
+    i = token - p.cu_seqlens[sequence];
+  } else if (p.seqlens_new != nullptr && s >= p.seqlens_new[b]) {
+    return make_longlong2(-1, -1);
+  }
+  const int before = p.seqlens[sequence];
+  const int64_t slot = static_cast<int64_t>(before) + i;
+  const int page = before < 0 || slot >= p.table.capacity() ? -1 : p.table.page_of(sequence, static_cast<int>(slot));
+  if (page < 0) {
+    if (p.status != nullptr) atomicCAS(p.status, 0, static_cast<int>(kPagedBadPage));
+    return make_longlong2(-1, -1);
+  }
+  const int row = p.table.page_size.mod(static_cast<int>(slot));
+  return make_longlong2(page * p.kos.outer + row * p.kos.row, page * p.vos.outer + row * p.vos.row);
+}
+
+template <bool BF16>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if constexpr (BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  float2 f;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.f32.f16 %0, lo;\n\tcvt.f32.f16 %1, hi;\n\t}" : "=f"(f.x), "=f"(f.y) : "r"(w));
+  return f;
+}
+
+// One head of one token: its rows in memory, and whether it is turned.
+struct Head {
+  const uint16_t* in;
+  uint16_t* out;   // null: not written
+  bool turned;
+};
+template <bool APPEND>
+__device__ __forceinline__ Head head_of(const RotaryParams& p, int b, int s, int h, const longlong2& row) {
+  Head r;
+  r.turned = true;
+  if (h < p.heads) {
+    r.in = static_cast<const uint16_t*>(p.q) + b * p.qs.outer + s * p.qs.row + h * p.qs.head;
+    r.out = static_cast<uint16_t*>(p.q_out) + b * p.qos.outer + s * p.qos.row + h * p.qos.head;
+    return r;
+  }
+  h -= p.heads;
+  if (!APPEND || h < p.heads_k) {
+    r.in = static_cast<const uint16_t*>(p.k) + b * p.ks.outer + s * p.ks.row + h * p.ks.head;
+    r.out = static_cast<uint16_t*>(p.k_out);
+    if constexpr (!APPEND) r.out += b * p.kos.outer + s * p.kos.row + h * p.kos.head;
+    else r.out = row.x < 0 ? nullptr : r.out + row.x + h * p.kos.head;
+    return r;
+  }
+  h -= p.heads_k;
+  r.in = static_cast<const uint16_t*>(p.v) + b * p.vs.outer + s * p.vs.row + h * p.vs.head;
+  r.out = row.y < 0 ? nullptr : static_cast<uint16_t*>(p.v_out) + row.y + h * p.vos.head;
+  r.turned = false;
+  return r;
+}
+
+// 16 bytes at a time: every row 16-byte aligned, pairs a multiple of 8. An item is 16 elements: 8 pairs, or 16 (at a head's end 8)
+// elements that are copied.
+template <bool BF16, bool NEIGHBOURS, bool APPEND>
+__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryParams p) {
+  extern __shared__ __align__(16) float s_turn[];  // [token][cos 0-3, cos 4-7, sin 0-3, sin 4-7][chunk of 8 pairs][4]
+  __shared__ longlong2 s_row[32];
+  const int tid = threadIdx.x;
+  const int chunks = p.pairs / 8, n = p.pairs;
+  early_wait();
+  early_trigger();
+  const int first = blockIdx.x * p.tokens_per_block;
+  const int tokens = min(p.tokens_per_block, p.tokens - first);
+  const int total = tokens * static_cast<int>(p.heads_all.d * p.items.d);
+
+  struct Item {
+    int token, b, s, h, c;
+  };
+  auto item = [&](int i) {
+    Item r;
+    const int row = p.items.div(i);
+    r.c = i - row * static_cast<int>(p.items.d);
+    r.token = p.heads_all.div(row);
+    r.h = row - r.token * static_cast<int>(p.heads_all.d);
+    const int t = first + r.token;
+    r.b = p.seqlen.div(t);
+    r.s = t - r.b * static_cast<int>(p.seqlen.d);
+    return r;
+  };
+  auto places = [&](const Item& r, bool turned, int& e0, int& e1) {
+    if (turned && r.c < chunks) {
+      e0 = NEIGHBOURS ? 16 * r.c : 8 * r.c;
+      e1 = NEIGHBOURS ? e0 + 8 : n + e0;
+    } else {  // behind the turned elements 16 at a time; in a head that is only copied from the start
+      e0 = 16 * r.c;
+      e1 = e0 + 8;
+    }
+  };
+  constexpr int kBatch = 4;
+  uint4 w0[kBatch], w1[kBatch];
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int i = i0 + u * kThreads;
+      if (i < total) {
+        const Item r = item(i);
+        const Head h = head_of<APPEND>(p, r.b, r.s, r.h, make_longlong2(0, 0));
+        int e0, e1;
+        places(r, h.turned, e0, e1);
+        w0[u] = *reinterpret_cast<const uint4*>(h.in + e0);
+        if (e1 < p.head_dim) w1[u] = *reinterpret_cast<const uint4*>(h.in + e1);
+      }
+    }
+  };
+  load(tid);
+  for (int i = tid; i < tokens * n; i += kThreads) {
+    const int token = i / n, pair = i - token * n;
+    const int t = first + token, b = p.seqlen.div(t);
+    const float2 cs = turn_of_pair(p, b, t - b * static_cast<int>(p.seqlen.d), pair);
+    const int at = ((token * 4 + (pair & 7) / 4) * chunks + pair / 8) * 4 + (pair & 3);
+    s_turn[at] = cs.x;
+    s_turn[at + 2 * chunks * 4] = cs.y;
+  }
+  if (APPEND && tid < tokens) {
+    const int t = first + tid, b = p.seqlen.div(t);
+    s_row[tid] = cache_row(p, t, b, t - b * static_cast<int>(p.seqlen.d));
+  }
+  __syncthreads();
+  for (int i0 = tid; i0 < total; i0 += kBatch * kThreads) {
+    if (i0 != tid) load(i0);
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int i = i0 + u * kThreads;
+      if (i >= total) break;
+      const Item r = item(i);
+      const Head h = head_of<APPEND>(p, r.b, r.s, r.h, APPEND ? s_row[r.token] : make_longlong2(0, 0));
+      if (APPEND && h.out == nullptr) continue;
+      int e0, e1;
+      places(r, h.turned, e0, e1);
+      uint32_t a[8] = {w0[u].x, w0[u].y, w0[u].z, w0[u].w, w1[u].x, w1[u].y, w1[u].z, w1[u].w};
+      if (h.turned && r.c < chunks) {
+        float cs[16];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float4 f = *reinterpret_cast<const float4*>(s_turn + ((r.token * 4 + k) * chunks + r.c) * 4);
+          cs[4 * k] = f.x;
+          cs[4 * k + 1] = f.y;
+          cs[4 * k + 2] = f.z;
+          cs[4 * k + 3] = f.w;
+        }
+        if constexpr (NEIGHBOURS) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float2 x = unpack2<BF16>(a[j]);
+            a[j] = pack2<BF16>(x.x * cs[j] - x.y * cs[8 + j], x.y * cs[j] + x.x * cs[8 + j]);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 x = unpack2<BF16>(a[j]), y = unpack2<BF16>(a[4 + j]);
+            const float c0 = cs[2 * j], c1 = cs[2 * j + 1], s0 = cs[8 + 2 * j], s1 = cs[9 + 2 * j];
+            a[j] = pack2<BF16>(x.x * c0 - y.x * s0, x.y * c1 - y.y * s1);
+            a[4 + j] = pack2<BF16>(y.x * c0 + x.x * s0, y.y * c1 + x.y * s1);
+          }
+        }
+      }
+      *reinterpret_cast<uint4*>(h.out + e0) = make_uint4(a[0], a[1], a[2], a[3]);
+      if (e1 < p.head_dim) *reinterpret_cast<uint4*>(h.out + e1) = make_uint4(a[4], a[5], a[6], a[7]);
+    }
+  }
+}
+
+// Any strides and any number of pairs, two bytes at a time: a block a token.
+template <bool BF16, bool APPEND>
+__global__ void __launch_bounds__(kThreads) rotary_any_kernel(const __grid_constant__ RotaryParams p) {
+  __shared__ float2 s_turn[128];
+  __shared__ longlong2 s_row;
+  const int tid = threadIdx.x, n = p.pairs;
+  early_wait();
+  early_trigger();
+  const int t = blockIdx.x, b = p.seqlen.div(t), s = t - b * static_cast<int>(p.seqlen.d);
+  for (int i = tid; i < n; i += kThreads) s_turn[i] = turn_of_pair(p, b, s, i);
+  if (tid == 0) s_row = APPEND ? cache_row(p, t, b, s) : make_longlong2(0, 0);
+  __syncthreads();
+  const longlong2 row = s_row;
+  const int heads = static_cast<int>(p.heads_all.d);
+  auto value = [](uint16_t x) { return unpack2<BF16>(x).x; };
+  for (int i = tid; i < heads * p.head_dim; i += kThreads) {
+    const int h = i / p.head_dim, e = i - h * p.head_dim;
+    const Head r = head_of<APPEND>(p, b, s, h, row);
+    if (r.out == nullptr) continue;
+    if (!r.turned || e >= 2 * n) {
+      r.out[e] = r.in[e];
+      continue;
+    }
+    const bool second = p.neighbours ? (e & 1) : e >= n;
+    const int pair = p.neighbours ? e >> 1 : second ? e - n : e;
+    const int other = p.neighbours ? e ^ 1 : second ? e - n : e + n;
+    const float2 cs = s_turn[pair];
+    const float x = value(r.in[e]), y = value(r.in[other]);
+    const float f = second ? x * cs.x + y * cs.y : x * cs.x - y * cs.y;
+    r.out[e] = static_cast<uint16_t>(pack2<BF16>(f, 0.f));
+  }
+}
+
+template <bool BF16, bool APPEND>
+cudaError_t pick(const RotaryParams& p, bool vectors, cudaStream_t stream) {
+  if (!vectors) return launch_grid(true, rotary_any_kernel<BF16, APPEND>, dim3(p.tokens), kThreads, 0, stream, p);
+  const int grid = (p.tokens + p.tokens_per_block - 1) / p.tokens_per_block;
+  const size_t smem = static_cast<size_t>(p.tokens_per_block) * p.pairs * 8;
+  if (p.neighbours) return launch_grid(true, rotary_kernel<BF16, true, APPEND>, dim3(grid), kThreads, smem, stream, p);
+  return launch_grid(true, rotary_kernel<BF16, false, APPEND>, dim3(grid), kThreads, smem, stream, p);
+}
+
+}  // namespace
+
+cudaError_t launch_rotary(const RotaryParams& p, bool bf16, bool append, bool vectors, cudaStream_t stream) {
+  if (p.tokens <= 0 || p.tokens_per_block <= 0 || p.tokens_per_block > 32 || p.pairs < 0 || p.pairs > 128) return cudaErrorInvalidValue;
+  if (append) return bf16 ? pick<true, true>(p, vectors, stream) : pick<false, true>(p, vectors, stream);
+  return bf16 ? pick<true, false>(p, vectors, stream) : pick<false, false>(p, vectors, stream);
+}
+
+}  // namespace fa2

@@ -65,11 +65,56 @@ class BwdOptions(C.Structure):
     ]
 
 
+class PagedCache(C.Structure):
+    _fields_ = [
+        ("size", C.c_int64), ("k", C.c_void_p), ("v", C.c_void_p), ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3),
+        ("attn_mass", C.c_void_p), ("block_table", C.c_void_p), ("block_table_stride", C.c_int64), ("seqlens_k", C.c_void_p),
+        ("num_pages", C.c_int32), ("page_size", C.c_int32), ("max_pages", C.c_int32), ("batch", C.c_int32),
+        ("heads_k", C.c_int32), ("head_dim", C.c_int32), ("dtype", C.c_int32), ("reserved", C.c_int32),
+    ]
+
+
+class RotaryArgs(C.Structure):
+    _fields_ = [
+        ("size", C.c_int64), ("q", C.c_void_p), ("q_out", C.c_void_p), ("k", C.c_void_p), ("k_out", C.c_void_p),
+        ("q_stride", C.c_int64 * 3), ("q_out_stride", C.c_int64 * 3), ("k_stride", C.c_int64 * 3),
+        ("k_out_stride", C.c_int64 * 3), ("positions", C.c_void_p), ("position_stride", C.c_int64 * 3),
+        ("inv_freq", C.c_void_p), ("position_bits", C.c_int32), ("dtype", C.c_int32), ("batch", C.c_int32),
+        ("seqlen", C.c_int32), ("heads", C.c_int32), ("heads_k", C.c_int32), ("head_dim", C.c_int32), ("axes", C.c_int32),
+        ("sections", C.c_int32 * 4), ("interleaved_axes", C.c_int32), ("interleaved_pairs", C.c_int32),
+        ("inverse", C.c_int32), ("reserved", C.c_int32),
+    ]
+
+
+class PagedAppendArgs(C.Structure):
+    _fields_ = [
+        ("size", C.c_int64), ("turn", C.POINTER(RotaryArgs)), ("cache", C.POINTER(PagedCache)), ("v", C.c_void_p),
+        ("v_stride", C.c_int64 * 3), ("cu_seqlens", C.c_void_p), ("seqlens_new", C.c_void_p),
+    ]
+
+
+class PagedFwdArgs(C.Structure):
+    _fields_ = [
+        ("size", C.c_int64), ("cache", C.POINTER(PagedCache)), ("q", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p),
+        ("q_stride", C.c_int64 * 3), ("o_stride", C.c_int64 * 3), ("seqlen_q", C.c_int32), ("heads", C.c_int32),
+        ("softmax_scale", C.c_float), ("window_left", C.c_int32), ("softcap", C.c_float), ("max_seqlen_k", C.c_int32),
+    ]
+
+
+class PagedEvictArgs(C.Structure):
+    _fields_ = [
+        ("size", C.c_int64), ("cache", C.POINTER(PagedCache)), ("dst_block_table", C.c_void_p),
+        ("dst_block_table_stride", C.c_int64), ("dst_max_pages", C.c_int32), ("budget", C.c_int32), ("recent", C.c_int32),
+        ("reserved", C.c_int32), ("seqlens_out", C.c_void_p), ("kept", C.c_void_p),
+    ]
+
+
 # Every symbol include/fa2_b200.h declares; the CPU test suite checks that the library exports them.
 EXPORTS = (
     "fa2_fwd", "fa2_fwd_with_workspace", "fa2_fwd_workspace_bytes", "fa2_varlen_fwd", "fa2_bwd_preprocess",
     "fa2_bwd_workspace_bytes", "fa2_bwd", "fa2_bwd_workspace_bytes_with_options", "fa2_bwd_with_options",
     "fa2_bwd_static", "fa2_bwd_static_status", "fa2_layout_is_addressable", "fa2_pack_16bit", "fa2_copy_16bit",
+    "fa2_rotary", "fa2_paged_append", "fa2_paged_fwd_workspace_bytes", "fa2_paged_fwd", "fa2_paged_evict",
     "fa2_last_error", "fa2_device_status", "fa2_sm_count",
 )
 
@@ -109,6 +154,13 @@ def load() -> C.CDLL:
             lib.fa2_bwd_static.restype = C.c_int
             lib.fa2_bwd_static_status.argtypes = [C.c_int]
             lib.fa2_bwd_static_status.restype = C.c_int
+        for name, args in (("fa2_rotary", RotaryArgs), ("fa2_paged_append", PagedAppendArgs), ("fa2_paged_evict", PagedEvictArgs)):
+            getattr(lib, name).argtypes = [C.POINTER(args), C.c_void_p]
+            getattr(lib, name).restype = C.c_int
+        lib.fa2_paged_fwd_workspace_bytes.argtypes = [C.POINTER(PagedFwdArgs)]
+        lib.fa2_paged_fwd_workspace_bytes.restype = C.c_int64
+        lib.fa2_paged_fwd.argtypes = [C.POINTER(PagedFwdArgs), C.c_void_p, C.c_int64, C.c_void_p]
+        lib.fa2_paged_fwd.restype = C.c_int
         lib.fa2_device_status.argtypes = [C.c_int]
         lib.fa2_device_status.restype = C.c_int
         lib.fa2_sm_count.argtypes = [C.c_int]

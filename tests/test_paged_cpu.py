@@ -1,0 +1,287 @@
+"""CPU: the index arithmetic of the operators on a paged cache (csrc/paged_index.h) through a small library around that header, and
+what their C entry points refuse before anything runs."""
+import ctypes as C
+import random
+import subprocess
+from pathlib import Path
+
+import pytest
+import torch
+
+ROOT = Path(__file__).resolve().parent.parent
+
+SHIM = r'''
+#include <cuda_runtime.h>
+#include "paged_index.h"
+using namespace fa2;
+extern "C" {
+int fast_div(int n, int d) { return make_div(d).div(n); }
+int fast_mod(int n, int d) { return make_div(d).mod(n); }
+int page_of(const int32_t* pages, int64_t stride, int max_pages, int num_pages, int page_size, int b, int slot) {
+  PageTable t;
+  t.pages = pages; t.stride = stride; t.max_pages = max_pages; t.num_pages = num_pages; t.page_size = make_div(page_size);
+  return t.page_of(b, slot);
+}
+int cut(int n, int64_t most) { return cut_length(n, most); }
+int first_tile(int n, int sq, int window, int tile) { return first_seen_tile(n, sq, window, tile); }
+int tiles(int n, int sq, int window, int tile) { return tiles_of(n, sq, window, tile); }
+int64_t begin(int64_t c, int64_t tiles, int64_t grid) { return share_begin(c, tiles, grid); }
+int owner(int64_t tile, int64_t tiles, int64_t grid) { return share_owner(tile, tiles, grid); }
+int axis(int i, int axes, const int32_t* sections, int turns) { return axis_of_pair(i, axes, sections, turns); }
+}
+'''
+
+
+@pytest.fixture(scope="module")
+def index(tmp_path_factory):
+    d = tmp_path_factory.mktemp("paged")
+    (d / "shim.cc").write_text(SHIM)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-shared", "-fPIC", f"-I{ROOT / 'kernels-community-rs_b200' / 'csrc'}",
+                    "-I/usr/local/cuda/include", str(d / "shim.cc"), "-o", str(d / "shim.so")], check=True)
+    lib = C.CDLL(str(d / "shim.so"))
+    lib.begin.restype = C.c_int64
+    lib.begin.argtypes = [C.c_int64] * 3
+    lib.owner.argtypes = [C.c_int64] * 3
+    lib.cut.argtypes = [C.c_int, C.c_int64]
+    return lib
+
+
+def test_division_by_multiplication(index):
+    rng = random.Random(1)
+    divisors = [1, 2, 3, 5, 7, 16, 17, 48, 100, 255, 256, 641, 65535, 65536, 2 ** 30 - 1, 2 ** 30, 2 ** 30 + 1, 2 ** 31 - 1]
+    for d in divisors + [rng.randrange(1, 2 ** 31) for _ in range(200)]:
+        around = [k * d + e for k in (0, 1, 2, (2 ** 31 - 1) // d) for e in (-1, 0, 1)]
+        for n in around + [2 ** 31 - 1, 2 ** 31 - 2] + [rng.randrange(2 ** 31) for _ in range(50)]:
+            if 0 <= n < 2 ** 31:
+                assert index.fast_div(n, d) == n // d and index.fast_mod(n, d) == n % d, (n, d)
+
+
+def test_pages_that_cannot_be_are_none(index):
+    """Entries outside the pool, and tokens outside the table's row, give no page; nothing behind the row is read."""
+    table = (C.c_int32 * 8)(3, -1, 7, 2 ** 31 - 1, 0, 8, -2 ** 31, 5)
+
+    def page(b, slot):
+        return index.page_of(table, C.c_int64(4), 4, 8, 10, b, slot)
+
+    assert [page(0, s) for s in (0, 9, 10, 20, 39)] == [3, 3, -1, 7, -1]
+    assert [page(1, s) for s in (0, 10, 29, 30)] == [0, -1, -1, 5]
+    assert [page(0, s) for s in (-1, -2 ** 31, 40, 2 ** 31 - 1)] == [-1] * 4
+    # a row of a table with room for more than 2^31 tokens
+    assert index.page_of(table, C.c_int64(4), 4, 8, 2 ** 30, 0, 2 ** 31 - 1) == -1
+    assert index.page_of(table, C.c_int64(4), 4, 8, 2 ** 30, 0, 2 ** 30 - 1) == 3
+
+
+def test_lengths_are_cut(index):
+    assert [index.cut(n, 100) for n in (-2 ** 31, -1, 0, 100, 101, 2 ** 31 - 1)] == [0, 0, 0, 100, 100, 100]
+    assert index.cut(2 ** 31 - 1, 2 ** 40) == 2 ** 31 - 1
+
+
+@pytest.mark.parametrize("tile", [64, 128])
+def test_tiles_hold_every_key_that_a_row_sees(index, tile):
+    for n in (0, 1, 63, 64, 65, 127, 128, 129, 1000, 4096, 2 ** 31 - 70000):
+        for sq in (1, 2, 5, 128):
+            for window in (-1, 0, 1, 63, 64, 500, 2 ** 31 - 70001):
+                first, count = index.first_tile(n, sq, window, tile), index.tiles(n, sq, window, tile)
+                lo = max(0, n - sq - window) if window >= 0 else 0
+                assert count >= 1 and first * tile <= lo and (lo - first * tile < tile)
+                assert (first + count) * tile >= n
+                if n > first * tile:
+                    assert (first + count - 1) * tile < n
+
+
+def test_shares_cover_the_tiles_once(index):
+    rng = random.Random(2)
+    for tiles, grid in [(1, 1), (1, 148), (147, 148), (148, 148), (149, 148), (5000, 148), (7, 3)] + \
+            [(rng.randrange(1, 3000), rng.randrange(1, 149)) for _ in range(50)]:
+        bounds = [index.begin(c, tiles, grid) for c in range(grid + 1)]
+        assert bounds[0] == 0 and bounds[-1] == tiles and sorted(bounds) == bounds
+        if tiles >= grid:  # the kernel takes no more CTAs than tiles: then each has some, and a unit's parts are neighbours'
+            assert all(a < b for a, b in zip(bounds, bounds[1:]))
+        for x in range(tiles):
+            c = index.owner(x, tiles, grid)
+            assert bounds[c] <= x < bounds[c + 1], (x, tiles, grid)
+    # long lists: products past 32 bits
+    tiles, grid = 2 ** 40 + 12345, 148
+    for c in (0, 1, 77, 147):
+        assert index.owner(index.begin(c, tiles, grid), tiles, grid) == c
+        assert index.owner(index.begin(c + 1, tiles, grid) - 1, tiles, grid) == c
+
+
+@pytest.mark.parametrize("sections", [(64,), (16, 24, 24), (24, 20, 20), (1, 0, 2, 1), (0, 5), (43, 21, 0)])
+def test_axes_of_the_pairs(index, sections):
+    n, axes = sum(sections), len(sections)
+    s = (C.c_int32 * 4)(*sections)
+    assert [index.axis(i, axes, s, 0) for i in range(n)] == [a for a, c in enumerate(sections) for _ in range(c)]
+    want = [0] * n
+    for a in range(1, axes):
+        want[a:axes * sections[a]:axes] = [a] * len(range(a, min(n, axes * sections[a]), axes))
+    assert [index.axis(i, axes, s, 1) for i in range(n)] == want
+
+
+# ---------------------------------------------------------------- the C entry points
+def _cache(**kw):
+    from flash_attn2_b200 import _cabi
+
+    c = _cabi.PagedCache(size=C.sizeof(_cabi.PagedCache), k=1 << 20, v=1 << 21, k_stride=(16 * 2 * 64, 2 * 64, 64),
+                         v_stride=(16 * 2 * 64, 2 * 64, 64), attn_mass=1 << 22, block_table=1 << 23, block_table_stride=4,
+                         seqlens_k=1 << 24, num_pages=8, page_size=16, max_pages=4, batch=2, heads_k=2, head_dim=64, dtype=_cabi.FA2_BF16)
+    for name, value in kw.items():
+        setattr(c, name, value)
+    return c
+
+
+def _turn(**kw):
+    from flash_attn2_b200 import _cabi
+
+    a = _cabi.RotaryArgs(size=C.sizeof(_cabi.RotaryArgs), q=1 << 20, q_out=1 << 21, k=1 << 22, k_out=1 << 23, positions=1 << 24,
+                         inv_freq=1 << 25, position_bits=64, dtype=_cabi.FA2_BF16, batch=2, seqlen=3, heads=4, heads_k=2, head_dim=64,
+                         axes=3, sections=(12, 10, 10))
+    for name, value in kw.items():
+        setattr(a, name, value)
+    return a
+
+
+def _fwd(cache=None, **kw):
+    from flash_attn2_b200 import _cabi
+
+    a = _cabi.PagedFwdArgs(size=C.sizeof(_cabi.PagedFwdArgs), cache=C.pointer(_cache() if cache is None else cache), q=1 << 20, out=1 << 21,
+                           lse=1 << 22, q_stride=(256, 256, 64), o_stride=(256, 256, 64), seqlen_q=1, heads=4, softmax_scale=0.1,
+                           window_left=-1)
+    for name, value in kw.items():
+        setattr(a, name, value)
+    return a
+
+
+def _refused(function, args, code, word, *more):
+    from flash_attn2_b200 import _cabi
+
+    lib = _cabi.load()
+    assert getattr(lib, function)(C.byref(args), *more) == code, lib.fa2_last_error()
+    assert word in lib.fa2_last_error().decode()
+
+
+BAD_CACHES = [(dict(size=8), -1, "size"), (dict(dtype=7), -2, "float16"), (dict(head_dim=60), -1, "head dim"), (dict(head_dim=264), -1, "head dim"),
+              (dict(num_pages=0), -1, "positive"), (dict(page_size=-1), -1, "positive"), (dict(max_pages=0), -1, "positive"),
+              (dict(batch=70000), -1, "65535"), (dict(heads_k=0), -1, "65535"), (dict(k=0), -1, "non-null"), (dict(block_table=0), -1, "non-null"),
+              (dict(k=(1 << 20) + 8), -1, "aligned"), (dict(v_stride=(2048, 100, 64)), -1, "multiples of 8"),
+              (dict(k_stride=(2048, -128, 64)), -1, "negative"), (dict(reserved=1), -1, "reserved")]
+
+
+@pytest.mark.parametrize("change,code,word", BAD_CACHES, ids=[str(c[0]) for c in BAD_CACHES])
+def test_bad_caches_are_refused(built_libs, change, code, word):
+    from flash_attn2_b200 import _cabi
+
+    cache = _cache(**change)
+    _refused("fa2_paged_fwd", _fwd(cache), code, word, None, 0, None)
+    evict = _cabi.PagedEvictArgs(size=C.sizeof(_cabi.PagedEvictArgs), cache=C.pointer(cache), dst_block_table=1 << 20, dst_max_pages=1,
+                                 budget=4, seqlens_out=1 << 20, kept=1 << 20)
+    _refused("fa2_paged_evict", evict, code, word, None)
+    append = _cabi.PagedAppendArgs(size=C.sizeof(_cabi.PagedAppendArgs), turn=C.pointer(_turn()), cache=C.pointer(cache), v=1 << 20)
+    _refused("fa2_paged_append", append, code, word, None)
+
+
+BAD_TURNS = [(dict(size=8), -1, "size"), (dict(dtype=9), -2, "float16"), (dict(head_dim=12), -1, "head dim"), (dict(axes=0), -1, "axes"),
+             (dict(axes=5), -1, "axes"), (dict(sections=(40, 1, 1)), -1, "sections"), (dict(sections=(0, 0, 0)), -1, "sections"),
+             (dict(sections=(-1, 9, 9)), -1, "sections"), (dict(sections=(2, 10, 10), interleaved_axes=1), -1, "turns"),
+             (dict(position_bits=16), -1, "position_bits"), (dict(positions=0), -1, "positions"), (dict(positions=(1 << 20) + 4), -1, "aligned"),
+             (dict(inv_freq=0), -1, "inv_freq"), (dict(q_out=0), -1, "q_out"), (dict(q=(1 << 20) + 1), -1, "aligned"),
+             (dict(batch=2 ** 20, seqlen=2 ** 12), -1, "batch"), (dict(heads=0), -1, "heads"), (dict(k_out=0), -1, "k_out"),
+             (dict(seqlen=-1), -1, "batch")]
+
+
+@pytest.mark.parametrize("change,code,word", BAD_TURNS, ids=[str(c[0]) for c in BAD_TURNS])
+def test_bad_turns_are_refused(built_libs, change, code, word):
+    _refused("fa2_rotary", _turn(**change), code, word, None)
+
+
+@pytest.mark.parametrize("change,code,word", [
+    (dict(turn=dict(heads_k=4)), -1, "cache's heads"), (dict(turn=dict(head_dim=72)), -1, "cache's heads"), (dict(turn=dict(dtype=0)), -2, "dtype"),
+    (dict(turn=dict(k=0)), -1, "k is null"), (dict(turn=dict(batch=3)), -1, "batch"), (dict(cu_seqlens=1 << 20), -1, "cu_seqlens"),
+    (dict(v=0), -1, "v must"), (dict(v=(1 << 20) + 1), -1, "v must"), (dict(size=8), -1, "size")], ids=str)
+def test_bad_appends_are_refused(built_libs, change, code, word):
+    from flash_attn2_b200 import _cabi
+
+    change = dict(change)
+    turn, cache = _turn(**change.pop("turn", {})), _cache()
+    a = _cabi.PagedAppendArgs(size=C.sizeof(_cabi.PagedAppendArgs), turn=C.pointer(turn), cache=C.pointer(cache), v=1 << 20)
+    for name, value in change.items():
+        setattr(a, name, value)
+    _refused("fa2_paged_append", a, code, word, None)
+
+
+@pytest.mark.parametrize("change,word", [
+    (dict(size=8), "size"), (dict(heads=3), "multiple"), (dict(heads=0), "multiple"), (dict(seqlen_q=-1), "seqlen_q"), (dict(seqlen_q=65), "128 query rows"),
+    (dict(softmax_scale=float("nan")), "softmax_scale"), (dict(softcap=-1.0), "softcap"), (dict(softcap=float("inf")), "softcap"),
+    (dict(max_seqlen_k=-1), "max_seqlen_k"), (dict(q=0), "non-null"), (dict(out=0), "non-null"), (dict(lse=0), "non-null"),
+    (dict(q=(1 << 20) + 2), "aligned"), (dict(o_stride=(256, 256, 60)), "multiples of 8")], ids=str)
+def test_bad_forwards_are_refused(built_libs, change, word):
+    _refused("fa2_paged_fwd", _fwd(**change), -1, word, None, 0, None)
+
+
+@pytest.mark.parametrize("change,word", [
+    (dict(size=8), "size"), (dict(budget=0), "budget"), (dict(recent=-1), "recent"), (dict(recent=5), "recent"), (dict(dst_block_table=0), "dst_block_table"),
+    (dict(dst_max_pages=0), "dst_block_table"), (dict(kept=0), "kept"), (dict(seqlens_out=0), "seqlens_out"), (dict(reserved=1), "reserved")], ids=str)
+def test_bad_evictions_are_refused(built_libs, change, word):
+    from flash_attn2_b200 import _cabi
+
+    cache = _cache()
+    a = _cabi.PagedEvictArgs(size=C.sizeof(_cabi.PagedEvictArgs), cache=C.pointer(cache), dst_block_table=1 << 20, dst_max_pages=1, budget=4,
+                             recent=1, seqlens_out=1 << 20, kept=1 << 20)
+    for name, value in change.items():
+        setattr(a, name, value)
+    _refused("fa2_paged_evict", a, -1, word, None)
+    without = _cache(attn_mass=None)
+    b = _cabi.PagedEvictArgs(size=C.sizeof(_cabi.PagedEvictArgs), cache=C.pointer(without), dst_block_table=1 << 20, dst_max_pages=1, budget=4,
+                             seqlens_out=1 << 20, kept=1 << 20)
+    _refused("fa2_paged_evict", b, -1, "attn_mass", None)
+
+
+def test_null_arguments_are_refused(built_libs):
+    from flash_attn2_b200 import _cabi
+
+    lib = _cabi.load()
+    assert lib.fa2_rotary(None, None) == lib.fa2_paged_append(None, None) == lib.fa2_paged_evict(None, None) == -1
+    assert lib.fa2_paged_fwd(None, None, 0, None) == -1 and lib.fa2_paged_fwd_workspace_bytes(None) == 0
+
+
+@pytest.mark.parametrize("struct,mirror", [("fa2_paged_cache", "PagedCache"), ("fa2_rotary_args", "RotaryArgs"),
+                                           ("fa2_paged_append_args", "PagedAppendArgs"), ("fa2_paged_fwd_args", "PagedFwdArgs"),
+                                           ("fa2_paged_evict_args", "PagedEvictArgs")])
+def test_ctypes_mirrors_follow_the_header(struct, mirror, tmp_path):
+    from flash_attn2_b200 import _cabi
+    from tests.test_boundary_cpu import _header_fields
+
+    cls = getattr(_cabi, mirror)
+    assert [(n, [str(t._length_)] if hasattr(t, "_length_") else []) for n, t in cls._fields_] == _header_fields(struct)
+    names = [n for n, _ in cls._fields_]
+    (tmp_path / "p.c").write_text('#include <stdio.h>\n#include <stddef.h>\n#include "fa2_b200.h"\nint main(){printf("%zu", sizeof(' + struct + "));" +
+                                  "".join(f'printf(" %zu", offsetof({struct}, {n}));' for n in names) + "return 0;}")
+    subprocess.run(["gcc", f"-I{ROOT / 'include'}", str(tmp_path / "p.c"), "-o", str(tmp_path / "p")], check=True)
+    got = [int(x) for x in subprocess.run([str(tmp_path / "p")], capture_output=True, text=True).stdout.split()]
+    assert got == [C.sizeof(cls)] + [getattr(cls, n).offset for n in names]
+
+
+def test_cpu_tensors_and_wrong_types_are_refused(built_libs):
+    import flash_attn2_b200 as fa
+
+    z = torch.zeros(1, 3, 2, 64, dtype=torch.bfloat16)
+    pos, freq, table, n = torch.zeros(1, 1, 3, dtype=torch.int32), torch.zeros(32), torch.zeros(1, 4, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    cache, mass = torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16), torch.zeros(4, 2, 16)
+    calls = [lambda: fa.rotary_axes_func(z, z, pos, freq, (32,)),
+             lambda: fa.paged_append(z, z, z, cache, cache.clone(), table, n, pos, freq, (32,)),
+             lambda: fa.paged_fwd(z, cache, cache, table, n), lambda: fa.paged_evict(cache, cache, mass, table, n, table, 4)]
+    for call in calls:
+        with pytest.raises(NotImplementedError):
+            call()
+    with pytest.raises(TypeError):
+        fa.rotary_axes_func(z, z, pos, freq, 32)
+    with pytest.raises(TypeError):
+        fa.rotary_axes_func(z, z, pos, freq, (32.0,))
+    with pytest.raises(TypeError):
+        fa.paged_fwd("q", cache, cache, table, n)
+    with pytest.raises(ValueError):
+        fa.rotary_axes_func(z, z, pos, freq, (1, 2, 3, 4, 5))
+    with pytest.raises(ValueError):
+        fa.rotary_axes_func(None, None, pos, freq, (32,))
+    with pytest.raises(TypeError):
+        fa.paged_evict(cache, cache, mass, table, n, table, 4.0)
