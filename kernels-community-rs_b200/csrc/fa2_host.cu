@@ -26,6 +26,7 @@ using fa2::fail;
 using fa2::g_error;
 using fa2::get_runtime;
 using fa2::kMaxDevices;
+using fa2::make_map;
 using fa2::Runtime;
 using fa2::bwd_takes_pairs;
 using fa2::bwd_wide_takes_pairs;
@@ -95,27 +96,6 @@ int get_runtime(int device, Runtime** out) {
   return FA2_OK;
 }
 
-DeviceScope::DeviceScope(const void* ptr) {
-  cudaGetDevice(&prev_);
-  device_ = prev_;
-  cudaPointerAttributes attr;
-  if (ptr != nullptr && cudaPointerGetAttributes(&attr, ptr) == cudaSuccess &&
-      (attr.type == cudaMemoryTypeDevice || attr.type == cudaMemoryTypeManaged) && attr.device >= 0)
-    device_ = attr.device;
-  else
-    cudaGetLastError();  // an unknown pointer is not an error of this call
-  // Also when it is current already: a thread that has made no runtime call yet (autograd's) has no context bound,
-  // and the driver's tensor-map encoder needs one.
-  cudaSetDevice(device_);
-}
-DeviceScope::~DeviceScope() {
-  if (device_ != prev_) cudaSetDevice(prev_);
-}
-
-}  // namespace fa2
-
-namespace {
-
 // 4-D map over [batch][rows][heads][D] with arbitrary (16-byte multiple) outer strides; the
 // box is one 128-byte swizzle line wide and `box_rows` rows tall.
 int make_map(CUtensorMap* m, const void* ptr, int dtype, int esize, int64_t d, int64_t heads, int64_t rows,
@@ -140,6 +120,27 @@ int make_map(CUtensorMap* m, const void* ptr, int dtype, int esize, int64_t d, i
   if (r != CUDA_SUCCESS) return fail(FA2_E_VALUE, "cannot build a TMA descriptor for %s (CUresult %d)", name, (int)r);
   return FA2_OK;
 }
+
+DeviceScope::DeviceScope(const void* ptr) {
+  cudaGetDevice(&prev_);
+  device_ = prev_;
+  cudaPointerAttributes attr;
+  if (ptr != nullptr && cudaPointerGetAttributes(&attr, ptr) == cudaSuccess &&
+      (attr.type == cudaMemoryTypeDevice || attr.type == cudaMemoryTypeManaged) && attr.device >= 0)
+    device_ = attr.device;
+  else
+    cudaGetLastError();  // an unknown pointer is not an error of this call
+  // Also when it is current already: a thread that has made no runtime call yet (autograd's) has no context bound,
+  // and the driver's tensor-map encoder needs one.
+  cudaSetDevice(device_);
+}
+DeviceScope::~DeviceScope() {
+  if (device_ != prev_) cudaSetDevice(prev_);
+}
+
+}  // namespace fa2
+
+namespace {
 
 // The same tensor with its head dim, a multiple of 64, as 64-column atoms: 5-D over [batch][heads][atoms][rows][64]. One load brings
 // 64 rows of two atoms, each atom's rows side by side.

@@ -155,12 +155,12 @@ int plan_fwd(const fa2_paged_fwd_args* a, int sm_count, FwdPlan* f) {
   const int64_t capacity = std::min<int64_t>(static_cast<int64_t>(c->max_pages) * c->page_size, kMostRows);
   f->most_keys = static_cast<int>(a->max_seqlen_k > 0 ? std::min<int64_t>(a->max_seqlen_k, capacity) : capacity);
   f->rows = a->seqlen_q * (a->heads / c->heads_k);
-  f->row_tiles = (f->rows + fa2::kPagedRows - 1) / fa2::kPagedRows;
-  const int tile = fa2::paged_tile_keys(c->head_dim);
-  const int64_t most_tiles = static_cast<int64_t>(c->batch) * c->heads_k * f->row_tiles * ((f->most_keys + static_cast<int64_t>(tile) - 1) / tile);
-  f->grid = static_cast<int>(std::min<int64_t>(sm_count, most_tiles));
+  const int unit_rows = fa2::paged_unit_rows(c->head_dim, f->rows);
+  f->row_tiles = (f->rows + unit_rows - 1) / unit_rows;
+  const int64_t most_tiles = static_cast<int64_t>(c->batch) * c->heads_k * f->row_tiles * ((f->most_keys + static_cast<int64_t>(fa2::kPagedTile) - 1) / fa2::kPagedTile);
+  f->grid = static_cast<int>(std::min<int64_t>(sm_count, (most_tiles + fa2::kPagedMinShare - 1) / fa2::kPagedMinShare));
   f->flag_bytes = round256(2 * static_cast<int64_t>(f->grid) * 8);
-  f->part_bytes = round256(2 * static_cast<int64_t>(f->grid) * fa2::paged_part_floats(c->head_dim) * 4);
+  f->part_bytes = round256(2 * static_cast<int64_t>(f->grid) * fa2::paged_part_floats(c->head_dim, f->rows) * 4);
   if (c->attn_mass != nullptr) {
     const int64_t rows = static_cast<int64_t>(c->batch) * c->heads_k * f->rows;
     f->score_stride = (f->most_keys + 15) / 16 * 16;
@@ -278,6 +278,15 @@ int fa2_paged_fwd(const fa2_paged_fwd_args* args, void* workspace, int64_t works
   p.vs = strides(c->v_stride);
   p.os = strides(args->o_stride);
   p.table = table_of(c);
+  p.tiled = c->page_size % fa2::kPagedTile == 0;
+  if (p.tiled) {
+    if ((rc = fa2::make_map(&p.tm_k, c->k, c->dtype, 2, c->head_dim, c->heads_k, c->page_size, c->num_pages, c->k_stride[2], c->k_stride[1],
+                            c->k_stride[0], 64, fa2::kPagedTile, "k")) != FA2_OK)
+      return rc;
+    if ((rc = fa2::make_map(&p.tm_v, c->v, c->dtype, 2, c->head_dim, c->heads_k, c->page_size, c->num_pages, c->v_stride[2], c->v_stride[1],
+                            c->v_stride[0], 64, fa2::kPagedTile, "v")) != FA2_OK)
+      return rc;
+  }
   p.seqlens = c->seqlens_k;
   p.most_keys = f.most_keys;
   p.batch = c->batch;

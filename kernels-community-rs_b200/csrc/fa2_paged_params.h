@@ -1,5 +1,6 @@
 // Kernel-side parameter blocks of the operators on a paged K/V cache.
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -44,6 +45,8 @@ struct RotaryParams {
 
 // Attention of the newest tokens over a paged cache (fwd_paged_sm100.cu).
 struct PagedParams {
+  CUtensorMap tm_k, tm_v;       // 4-D: (D, heads, rows of a page, pages), box (64, 1, 16, 1); used where tiled
+  int tiled;                    // page_size is a multiple of 16
   const void *q, *k, *v;
   void* o;
   float* lse;                   // [batch, heads, seqlen_q]
@@ -53,7 +56,7 @@ struct PagedParams {
   int most_keys;                // longer sequences are cut to it
   int batch, heads, heads_k, seqlen_q, head_dim;
   FastDiv group;                // heads / heads_k
-  int rows, row_tiles;          // seqlen_q * group, in tiles of 16
+  int rows, row_tiles;          // seqlen_q * group, in tiles of paged_unit_rows
   int window;
   float scale, scale_log2, softcap;
   float* partials;              // 2 slots per CTA
@@ -81,12 +84,15 @@ struct EvictParams {
 
 cudaError_t launch_rotary(const RotaryParams& p, bool bf16, bool append, bool vectors, cudaStream_t stream);
 
-constexpr int kPagedRows = 16;       // query rows of a unit
 constexpr int kPagedMaxRows = 128;   // query rows per kv head
-// Keys that a CTA takes at a time.
-inline int paged_tile_keys(int head_dim) { return head_dim > 128 ? 64 : 128; }
-// Floats of a partial result: O of 16 rows, their maxima and sums.
-inline int64_t paged_part_floats(int head_dim) { return kPagedRows * (static_cast<int64_t>((head_dim + 63) / 64 * 64) + 2); }
+constexpr int kPagedTile = 16;       // keys of a tile
+constexpr int kPagedMinShare = 4;    // tiles of a CTA's share at least, where there are that many
+// Query rows of a unit: what the accumulators of 64-column parts leave registers for.
+inline int paged_unit_rows(int head_dim, int rows) { return rows <= 8 ? 8 : rows <= 16 || head_dim > 128 ? 16 : 32; }
+// Floats of a partial result: O of a unit's rows, their maxima and sums.
+inline int64_t paged_part_floats(int head_dim, int rows) {
+  return paged_unit_rows(head_dim, rows) * (static_cast<int64_t>((head_dim + 63) / 64 * 64) + 2);
+}
 cudaError_t launch_fwd_paged(const PagedParams& p, int grid, bool bf16, cudaStream_t stream);
 cudaError_t launch_paged_mass(const PagedParams& p, int sm_count, cudaStream_t stream);
 

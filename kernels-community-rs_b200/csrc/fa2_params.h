@@ -23,6 +23,7 @@ enum WaitSite : int {
   kWaitBwd = 50,
   kWaitDecode = 80,
   kWaitBwdDq = 90,
+  kWaitPaged = 95,
 };
 
 constexpr int kMaxStreamBlocks = 64;   // 256-row query blocks of a head in a forward that shares tiles between CTAs

@@ -1,5 +1,7 @@
 // What the host files of the C ABI share: the error message, the state of a device, and the scope of a call's device.
 #pragma once
+#include <cuda.h>
+#include <stdint.h>
 
 namespace fa2 {
 
@@ -19,6 +21,11 @@ struct Runtime {
   int* status = nullptr;  // device status word
 };
 int get_runtime(int device, Runtime** out);
+
+// A tensor map over [batch][rows][heads][D] of 16-bit (dtype 2: fp32) elements; strides in elements, boxes of box_inner columns and
+// box_rows rows, 128-byte swizzle. The runtime has to be there.
+int make_map(CUtensorMap* m, const void* ptr, int dtype, int esize, int64_t d, int64_t heads, int64_t rows, int64_t batch, int64_t head_stride,
+             int64_t row_stride, int64_t batch_stride, int box_inner, int box_rows, const char* name);
 
 // Makes the device that owns `ptr` current for the lifetime of the object and restores the caller's
 // device afterwards, as the reference binds the context of q before every launch

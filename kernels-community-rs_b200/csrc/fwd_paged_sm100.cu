@@ -29,35 +29,41 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-template <int A>  // 64-column parts of the head dim
+template <int A, int NT>  // 64-column parts of the head dim; 8-row tiles of a unit
 struct Cfg {
   static constexpr int D = A * 64;
-  static constexpr int kWarps = A > 2 ? 4 : 8;
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kWarps = A == 1 ? (NT == 1 ? 14 : NT == 2 ? 12 : 8) : A == 2 ? (NT == 1 ? 10 : 8) : A == 3 ? 7 : 5;
   static constexpr int kThreads = kWarps * 32;
-  static constexpr int kTileKeys = kWarps * 16;
-  static constexpr int kPieces = 8 * A;                  // 16-byte pieces a lane copies for 16 keys: K and V
-  static constexpr int kStageBytes = kPieces * 32 * 16;  // of a warp
-  static constexpr int kStages = A == 1 ? 5 : A == 3 ? 4 : 3;
+  // A tile's 16 rows of K, then of V: 64 columns at a time, rows of 128 bytes whose 16-byte pieces are swizzled by the row.
+  static constexpr int kPart = 2048;
+  static constexpr int kVOff = A * kPart, kStageBytes = 2 * A * kPart;  // of a warp
+  static constexpr int kStages = A == 1 ? (NT == 4 ? 5 : 3) : 2;
   static constexpr int kQueueBytes = kWarps * kStages * kStageBytes;
-  static constexpr int kRowFloats = D + 4;               // a row of a warp's O when the warps' parts become one
-  static_assert(kPagedRows * kRowFloats * 4 <= kStages * kStageBytes, "the parts take the place of the queue");
-  static constexpr int kSmemBytes = kQueueBytes;
-  static_assert(kSmemBytes <= 227 * 1024 - 4096, "shared memory");
+  static constexpr bool kQInRegs = A * NT <= 4;          // else its fragments stay in shared memory
+  static constexpr int kQBytes = kQInRegs ? 0 : NT * A * 2 * 512;
+  static constexpr int kRowFloats = D + 4;               // a row of a warp's O when the warps' parts become one, 8 rows at a time
+  static constexpr int kPartOff = kQueueBytes + kQBytes, kPartBytes = kWarps * 8 * kRowFloats * 4;
+  static constexpr int kBarOff = kPartOff + kPartBytes;
+  static constexpr int kSmemBytes = kBarOff + kWarps * kStages * 8;
+  static_assert(kSmemBytes <= 227 * 1024 - 6144, "shared memory");
 };
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
   const int bytes = there ? 16 : 0;  // 0: zeroes
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copies_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// An arrival of this thread at a barrier, once its copies so far are there.
+__device__ __forceinline__ void copies_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 __device__ __forceinline__ uint4 lds16(uint32_t at) {
   uint4 w;
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(at) : "memory");
   return w;
+}
+__device__ __forceinline__ void sts16(uint32_t at, uint4 w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
 }
 template <bool BF16>
 __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
@@ -92,26 +98,59 @@ __device__ __forceinline__ bool not_finite(uint32_t w) {
 // exp2(m - m_tot) with m = -inf (a part that saw no key) giving 0 also when m_tot = -inf.
 __device__ __forceinline__ float part_scale(float m, float m_tot) { return m == -INFINITY ? 0.f : ex2(m - m_tot); }
 
-// A unit: 16 query rows of a kv head of a sequence, and the part of its key tiles that a share has.
+// The transpose of an 8 x 8 matrix of 16-bit numbers, two of a row in each lane.
+__device__ __forceinline__ uint32_t transposed(uint32_t w) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(w));
+  return r;
+}
+
+// A unit: up to 8 NT query rows of a kv head of a sequence, and the part of its 16-key tiles that a share has.
 struct Segment {
   int b, hk, rt;       // sequence, kv head, row tile
+  int unit;            // within the sequence
   int length;          // keys of the sequence
   int first, tiles;    // its key tiles [first, first + tiles)
+  int j0, j1;          // the share's
+  int64_t start;       // list index of the unit's first tile
+  int end_all, begin_all;  // keys outside [begin_all, end_all) are seen by no row
+};
+// A unit of which this CTA has left a part in the workspace.
+struct Pending {
+  int b, hk, rt, tiles;
+  int64_t start;
 };
 
-template <int A, bool BF16>
-__global__ void __launch_bounds__(Cfg<A>::kThreads, 1) fwd_paged_kernel(const __grid_constant__ PagedParams p) {
-  using C = Cfg<A>;
-  constexpr int D = C::D, W = C::kWarps, kKeys = C::kTileKeys;
-  extern __shared__ __align__(128) uint8_t smem[];
+// TILED: pages are whole tiles, so that a tile is one TMA box for each 64 columns of K and of V. Otherwise its rows lie in two or more
+// pages, and are copied 16 bytes at a time.
+template <int A, int NT, bool BF16, bool TILED>
+__global__ void __launch_bounds__((Cfg<A, NT>::kThreads), 1) fwd_paged_kernel(const __grid_constant__ PagedParams p) {
+  using C = Cfg<A, NT>;
+  constexpr int D = C::D, W = C::kWarps, R = C::kRows, kStages = C::kStages;
+  extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ int64_t s_sum[W];
   __shared__ int64_t s_before;        // tiles of the sequences before s_first
-  __shared__ int s_first;
-  __shared__ float s_m[W][kPagedRows], s_l[W][kPagedRows];
-  __shared__ uint32_t s_seen[W][C::kStages];
-  __shared__ int s_last;
+  __shared__ int s_first, s_length;   // ... and its length
+  __shared__ float s_m[W][8], s_l[W][8];
+  __shared__ Pending s_pending[2];
+  __shared__ int2 s_parts[2];   // of a pending unit: its first CTA, and how many there are if all are done, or 0
+  __shared__ int s_abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t4 = lane & 3;
+  uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + C::kBarOff) + warp * kStages;  // this warp's
+  const WaitCtl ctl{&s_abort};
+  if (tid == 0) s_abort = 0;
+  if (lane < kStages) mbar_init(&bars[lane], TILED ? 1 : 32);
+  mbar_fence_init();
+  if (TILED && tid == 0) {
+    tma_prefetch_desc(&p.tm_k);
+    tma_prefetch_desc(&p.tm_v);
+  }
+  if (tid == 0) {
+    s_first = 0;
+    s_before = 0;
+    s_length = 0;
+  }
   early_wait();
   early_trigger();
 
@@ -123,470 +162,549 @@ __global__ void __launch_bounds__(Cfg<A>::kThreads, 1) fwd_paged_kernel(const __
     if (n > most && p.status != nullptr) atomicCAS(p.status, 0, static_cast<int>(kPagedTooLong));
     return cut_length(n, most);
   };
-  auto tiles_in = [&](int b) { return tiles_of(length_of(b), p.seqlen_q, p.window, kKeys); };
-  int64_t mine = 0;
-  for (int b = tid; b < p.batch; b += C::kThreads) mine += tiles_in(b);
+  auto list_of = [&](int length) { return static_cast<int64_t>(tiles_of(length, p.seqlen_q, p.window, kPagedTile)) * units_per_seq; };
+  // Sum over the threads up to this one, and over all.
+  auto scan = [&](int64_t x, int64_t& all) {
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
-  if (lane == 0) s_sum[warp] = mine;
-  __syncthreads();
-  int64_t n_tiles = 0;
-#pragma unroll
-  for (int w = 0; w < W; ++w) n_tiles += s_sum[w];
-  n_tiles *= units_per_seq;
-  const int64_t ctas = min(n_tiles, static_cast<int64_t>(gridDim.x));  // none of them has nothing: a unit's parts are neighbours' parts
-  if (blockIdx.x >= ctas) return;
-  const int64_t lo = share_begin(blockIdx.x, n_tiles, ctas), hi = share_begin(blockIdx.x + 1, n_tiles, ctas);
-  if (tid == 0) {
-    s_first = 0;
-    s_before = 0;
-  }
-  // the sequence that tile lo belongs to: its number of tiles before reaches lo last
-  {
-    int64_t carry = 0;
-    for (int b0 = 0; b0 < p.batch; b0 += C::kThreads) {
-      const int b = b0 + tid;
-      const int64_t n = b < p.batch ? static_cast<int64_t>(tiles_in(b)) * units_per_seq : 0;
-      int64_t x = n;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, x, d);
-        if (lane >= d) x += y;
-      }
-      __syncthreads();
-      if (lane == 31) s_sum[warp] = x;
-      __syncthreads();
-      int64_t before = carry, all = 0;
-#pragma unroll
-      for (int w = 0; w < W; ++w) {
-        if (w < warp) before += s_sum[w];
-        all += s_sum[w];
-      }
-      before += x - n;
-      if (before <= lo && lo < before + n) {
-        s_first = b;
-        s_before = before;
-      }
-      carry += all;
-      if (carry > lo) break;
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, x, d);
+      if (lane >= d) x += y;
     }
     __syncthreads();
-  }
+    if (lane == 31) s_sum[warp] = x;
+    __syncthreads();
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      if (w == warp) x += all;
+      all += s_sum[w];
+    }
+    return x;
+  };
   Segment seg;
-  seg.b = s_first;
-  int64_t seg_start;  // list index of the segment's unit
-  int unit;           // within the sequence
+  int64_t n_tiles, ctas, lo, hi;
+  {
+    const int length = tid < p.batch ? length_of(tid) : 0;
+    int64_t n = tid < p.batch ? list_of(length) : 0, all;
+    int64_t upto = scan(n, all);
+    n_tiles = all;
+    if (p.batch > C::kThreads) {
+      int64_t more = 0, rest;
+      for (int b = tid + C::kThreads; b < p.batch; b += C::kThreads) more += list_of(length_of(b));
+      scan(more, rest);
+      n_tiles += rest;
+    }
+    // No CTA has nothing (a unit's parts are neighbours' parts), and none has less than a few tiles where there are more.
+    ctas = max(min((n_tiles + kPagedMinShare - 1) / kPagedMinShare, static_cast<int64_t>(gridDim.x)), static_cast<int64_t>(1));
+    if (blockIdx.x >= ctas) return;  // no copy has been started
+    lo = share_begin(blockIdx.x, n_tiles, ctas);
+    hi = share_begin(blockIdx.x + 1, n_tiles, ctas);
+    // the sequence that tile lo belongs to: its number of tiles before reaches lo last
+    auto look = [&](int b, int seq_length) {
+      if (upto - n <= lo && lo < upto) {
+        s_first = b;
+        s_before = upto - n;
+        s_length = seq_length;
+      }
+    };
+    look(tid, length);
+    for (int b0 = C::kThreads; b0 < p.batch && all <= lo; b0 += C::kThreads) {
+      const int b = b0 + tid, seq_length = b < p.batch ? length_of(b) : 0;
+      const int64_t before = all;
+      n = b < p.batch ? list_of(seq_length) : 0;
+      upto = scan(n, all) + before;
+      all += before;
+      look(b, seq_length);
+    }
+    __syncthreads();
+    seg.b = s_first;
+    seg.start = s_before;
+    seg.length = s_length;
+  }
   auto open_sequence = [&]() {
-    seg.length = length_of(seg.b);
-    seg.first = first_seen_tile(seg.length, p.seqlen_q, p.window, kKeys);
-    seg.tiles = tiles_of(seg.length, p.seqlen_q, p.window, kKeys);
+    seg.first = first_seen_tile(seg.length, p.seqlen_q, p.window, kPagedTile);
+    seg.tiles = tiles_of(seg.length, p.seqlen_q, p.window, kPagedTile);
+    seg.end_all = seg.length;
+    seg.begin_all = p.window < 0 ? 0 : max(0, seg.length - p.seqlen_q - p.window);
+  };
+  // The part of the unit that begins at seg.start which lies in [x, hi).
+  auto open_unit = [&](int64_t x) {
+    seg.hk = seg.unit / p.row_tiles;
+    seg.rt = seg.unit - seg.hk * p.row_tiles;
+    seg.j0 = static_cast<int>(x - seg.start);
+    seg.j1 = static_cast<int>(min(static_cast<int64_t>(seg.tiles), hi - seg.start));
   };
   open_sequence();
-  unit = static_cast<int>(min((lo - s_before) / seg.tiles, static_cast<int64_t>(units_per_seq - 1)));
-  seg_start = s_before + static_cast<int64_t>(unit) * seg.tiles;
+  {
+    const int64_t before = lo - seg.start;
+    seg.unit = static_cast<int>(before < (1ll << 31) ? static_cast<uint32_t>(before) / static_cast<uint32_t>(seg.tiles) : before / seg.tiles);
+    seg.unit = min(seg.unit, units_per_seq - 1);
+    seg.start += static_cast<int64_t>(seg.unit) * seg.tiles;
+  }
+  open_unit(lo);
 
-  const uint32_t queue = smem_u32(smem) + warp * (C::kStages * C::kStageBytes) + lane * 16;
+  const uint32_t queue = smem_u32(smem) + warp * (kStages * C::kStageBytes);
+  const uint32_t q_smem = smem_u32(smem) + C::kQueueBytes + lane * 16;
   const float inv_cap = p.softcap > 0.f ? p.scale / p.softcap : 0.f;
   const float cap_l2 = p.softcap * kLog2e;
+  const int group = static_cast<int>(p.group.d);
+  // Where this lane's pieces lie in 64 columns of a stage. K: pieces 2 t4 and 2 t4 + 1 of key g (of key g + 8 1024 bytes further); V:
+  // piece g of keys 2 t4 and 2 t4 + 1 (of keys 2 t4 + 8 and + 9 1024 bytes further). Of the eight lanes that a shared-memory access
+  // serves at once no two have the same banks: even pieces of two rows, or two pieces of four even rows.
+  const uint32_t k_at[2] = {static_cast<uint32_t>(g * 128 + ((2 * t4 ^ g) << 4)), static_cast<uint32_t>(g * 128 + ((2 * t4 + 1 ^ g) << 4))};
+  const uint32_t v_at[2] = {static_cast<uint32_t>(C::kVOff + 2 * t4 * 128 + ((g ^ 2 * t4) << 4)),
+                            static_cast<uint32_t>(C::kVOff + (2 * t4 + 1) * 128 + ((g ^ (2 * t4 + 1)) << 4))};
+  int stage = 0, phase = 0;                             // the next one to be read
 
-  for (int64_t x = lo; x < hi;) {
-    seg.hk = unit / p.row_tiles;
-    seg.rt = unit - seg.hk * p.row_tiles;
-    const int j0 = static_cast<int>(x - seg_start);
-    const int j1 = static_cast<int>(min(static_cast<int64_t>(seg.tiles), hi - seg_start));
-    // Rows of this thread: query and head.
-    const int r0 = seg.rt * 16 + g, r1 = r0 + 8;
-    const int q0 = p.group.div(r0), q1 = p.group.div(r1);
-    const int group = static_cast<int>(p.group.d);
-    const int rows = min(kPagedRows, p.rows - seg.rt * 16);
-    const int end_all = seg.length;                          // keys from here on are seen by no row
-    const int begin_all = p.window < 0 ? 0 : max(0, static_cast<int>(max(static_cast<int64_t>(seg.length) - p.seqlen_q - p.window, static_cast<int64_t>(0))));
-    // What each row sees: [lo, hi).
-    const int hi0 = seg.length - p.seqlen_q + q0 + 1, hi1 = seg.length - p.seqlen_q + q1 + 1;
-    const int lo0 = p.window < 0 ? 0 : hi0 - 1 - p.window, lo1 = p.window < 0 ? 0 : hi1 - 1 - p.window;
+  // ---- copies of 16 keys of the present segment
+  auto first_key = [&](int j) { return (seg.first + j) * kPagedTile; };
+  // The page of a tile (TILED), or of key `lane % 16` of it; -1: there is none, or no row sees it.
+  auto look_up = [&](int j) {
+    const int key = first_key(j) + (TILED ? 0 : lane & 15);
+    if (j >= seg.j1 || key >= seg.end_all || (!TILED && key < seg.begin_all)) return -1;
+    const int page = p.table.pages[seg.b * p.table.stride + p.table.page_size.div(key)];
+    if (static_cast<uint32_t>(page) < static_cast<uint32_t>(p.table.num_pages)) return page;
+    if (p.status != nullptr) atomicCAS(p.status, 0, static_cast<int>(kPagedBadPage));
+    return -1;
+  };
+  // Starts the copies of tile j into a stage that every lane has read, and returns a bit for each of its keys that some row sees.
+  auto issue = [&](int j, int page, int to_stage) {
+    const int key0 = first_key(j);
+    const uint32_t at = queue + to_stage * C::kStageBytes;
+    uint32_t seen;
+    if constexpr (TILED) {
+      seen = page < 0 ? 0u : bit_range(seg.begin_all - key0, min(seg.end_all - key0, 16));
+      if (elect_one()) {
+        mbar_expect_tx(&bars[to_stage], page < 0 ? 0 : C::kStageBytes);
+        if (page >= 0) {
+          const int row = p.table.page_size.mod(key0);
+#pragma unroll
+          for (int i = 0; i < A; ++i) {
+            tma_load_4d(smem + (at - smem_u32(smem)) + i * C::kPart, &p.tm_k, &bars[to_stage], i * 64, seg.hk, row, page);
+            tma_load_4d(smem + (at - smem_u32(smem)) + C::kVOff + i * C::kPart, &p.tm_v, &bars[to_stage], i * 64, seg.hk, row, page);
+          }
+        }
+      }
+      __syncwarp();
+    } else {
+      seen = __ballot_sync(0xffffffffu, page >= 0) & 0xffffu;
+      const int row = p.table.page_size.mod(key0 + (lane & 15));
+      const int64_t k_row = page < 0 ? 0 : page * p.ks.outer + row * p.ks.row;
+      const int64_t v_row = page < 0 ? 0 : page * p.vs.outer + row * p.vs.row;
+      // Neighbouring lanes take neighbouring pieces of a row; what is not there is zero.
+#pragma unroll
+      for (int i = 0; i < A * 4; ++i) {
+        const int r = (lane + 32 * i) / (A * 8), c = lane + 32 * i - r * (A * 8);
+        const bool there = (seen >> r & 1) && c * 8 < p.head_dim;
+        const uint32_t to = at + (c >> 3) * C::kPart + r * 128 + (((c ^ r) & 7) << 4);
+        const int64_t k_from = __shfl_sync(0xffffffffu, k_row, r) + c * 8, v_from = __shfl_sync(0xffffffffu, v_row, r) + c * 8;
+        copy16(to, static_cast<const uint16_t*>(p.k) + seg.hk * p.ks.head + (there ? k_from : 0), there);
+        copy16(to + C::kVOff, static_cast<const uint16_t*>(p.v) + seg.hk * p.vs.head + (there ? v_from : 0), there);
+      }
+      copies_arrive(&bars[to_stage]);
+    }
+    return seen;
+  };
+  uint32_t seen_of[kStages];  // of the tiles in the queue, the oldest first
+  int next_page;              // of the tile behind them
+  // Fills the queue with the segment's first tiles.
+  auto fill = [&]() {
+    int page[kStages];
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) page[i] = look_up(seg.j0 + warp + i * W);
+    next_page = look_up(seg.j0 + warp + kStages * W);
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) {
+      seen_of[i] = 0;
+      if (seg.j0 + warp + i * W < seg.j1) seen_of[i] = issue(seg.j0 + warp + i * W, page[i], stage + i < kStages ? stage + i : stage + i - kStages);
+    }
+  };
+  fill();
+
+  // Four columns of a row's end, and with the first of them the LSE (+inf for a row that saw no key) and what turns scores into weights.
+  auto store_row = [&](int b, int hk, int row, int col, const float4& acc, float top, float total) {
+    const int q = p.group.div(row), h = hk * group + row - q * group;
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    if (col < p.head_dim)
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.o) + b * p.os.outer + q * p.os.row + h * p.os.head + col) =
+          make_uint2(pack2<BF16>(acc.x * inv, acc.y * inv), pack2<BF16>(acc.z * inv, acc.w * inv));
+    if (col == 0) {
+      p.lse[(static_cast<int64_t>(b) * p.heads + h) * p.seqlen_q + q] = total == 0.f ? INFINITY : (top + log2f(total)) * kLn2;
+      if (p.stats != nullptr) __stcg(p.stats + (static_cast<int64_t>(b) * p.heads_k + hk) * p.rows + row, make_float2(top, inv));
+    }
+  };
+  constexpr int kSlot = R * (D + 2);  // floats of a part in the workspace
+
+  int n_pending = 0;
+  for (bool more = true; more;) {
+    const int row0 = seg.rt * R;
+    const int rows = min(R, p.rows - row0);
     // Keys [same_lo, same_hi) are seen by every row of the call.
     const int same_hi = seg.length - p.seqlen_q + 1;
     const int same_lo = p.window < 0 ? 0 : seg.length - 1 - p.window;
+    // What query q sees: keys [from(q), to(q)).
+    auto to = [&](int q) { return seg.length - p.seqlen_q + q + 1; };
+    auto from = [&](int q) { return p.window < 0 ? 0 : to(q) - 1 - p.window; };
 
-    // ---- Q: pieces t4 + 4 i of rows g and g + 8 as A fragments of k-steps 2 i and 2 i + 1
-    uint32_t qf[A * 4][4];
-    {
-      const uint16_t* base = static_cast<const uint16_t*>(p.q) + seg.b * p.qs.outer + (seg.hk * group) * p.qs.head;
-      const uint16_t* a0 = base + q0 * p.qs.row + (r0 - q0 * group) * p.qs.head;
-      const uint16_t* a1 = base + q1 * p.qs.row + (r1 - q1 * group) * p.qs.head;
+    // ---- Q: of row g of each 8-row tile the pieces that K has, as B fragments of k-steps 2 i and 2 i + 1
+    uint4 qf[C::kQInRegs ? NT * A * 2 : 1];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      if (!C::kQInRegs && n != warp) continue;  // every warp needs the same
+      const int r = row0 + 8 * n + g, q = p.group.div(r);
+      const uint16_t* base = static_cast<const uint16_t*>(p.q) + seg.b * p.qs.outer + q * p.qs.row + (seg.hk * group + r - q * group) * p.qs.head;
 #pragma unroll
       for (int i = 0; i < A * 2; ++i) {
-        const int e = (t4 + 4 * i) * 8;
-        uint4 w0 = make_uint4(0, 0, 0, 0), w1 = w0;
-        if (r0 < p.rows && e < p.head_dim) w0 = *reinterpret_cast<const uint4*>(a0 + e);
-        if (r1 < p.rows && e < p.head_dim) w1 = *reinterpret_cast<const uint4*>(a1 + e);
-        qf[2 * i][0] = w0.x, qf[2 * i][1] = w1.x, qf[2 * i][2] = w0.y, qf[2 * i][3] = w1.y;
-        qf[2 * i + 1][0] = w0.z, qf[2 * i + 1][1] = w1.z, qf[2 * i + 1][2] = w0.w, qf[2 * i + 1][3] = w1.w;
+        const int e = (8 * (i >> 1) + 2 * t4 + (i & 1)) * 8;
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (r < p.rows && e < p.head_dim) w = *reinterpret_cast<const uint4*>(base + e);
+        if constexpr (C::kQInRegs) qf[n * (A * 2) + i] = w;
+        else sts16(q_smem + (n * (A * 2) + i) * 512, w);
       }
     }
+    if constexpr (!C::kQInRegs) __syncthreads();
 
-    // ---- copies of 16 keys
-    const uint16_t* k_head = static_cast<const uint16_t*>(p.k) + seg.hk * p.ks.head;
-    const uint16_t* v_head = static_cast<const uint16_t*>(p.v) + seg.hk * p.vs.head;
-    auto first_key = [&](int j) { return (seg.first + j) * kKeys + warp * 16; };
-    // The page of key `lane % 16` of the warp's 16, looked up one step ahead of its copies.
-    auto look_up = [&](int j) {
-      const int key = first_key(j) + (lane & 15);
-      if (j >= j1 || key >= end_all || key < begin_all) return -1;
-      const int page = p.table.page_of(seg.b, key);
-      if (page < 0 && p.status != nullptr) atomicCAS(p.status, 0, static_cast<int>(kPagedBadPage));
-      return page;
-    };
-    int next_page = look_up(j0);
-    auto issue = [&](int j, int stage) {
-      const int page = next_page;
-      const uint32_t seen = __ballot_sync(0xffffffffu, page >= 0) & 0xffffu;
-      if (lane == 0) s_seen[warp][stage] = seen;
-      if (j < j1) {
-        const int row = p.table.page_size.mod(first_key(j) + (lane & 15));
-        const int64_t k_row = page < 0 ? 0 : page * p.ks.outer + row * p.ks.row;
-        const int64_t v_row = page < 0 ? 0 : page * p.vs.outer + row * p.vs.row;
-        const uint32_t at = queue + stage * C::kStageBytes;
+    // Rows of this thread: row0 + 8 n + 2 t4 + e.
+    float m[NT][2], l[NT][2];
+    float o[A * 4][NT][4];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int key = g + 8 * half;
-          const uint16_t* src = k_head + __shfl_sync(0xffffffffu, k_row, key) + t4 * 8;
-          const bool there = seen >> key & 1;
+    for (int n = 0; n < NT; ++n) {
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.f;
 #pragma unroll
-          for (int i = 0; i < A * 2; ++i) {
-            const bool in = there && (t4 + 4 * i) * 8 < p.head_dim;
-            copy16(at + (half * (A * 2) + i) * 512, in ? src + i * 32 : k_head, in);
-          }
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int key = 2 * t4 + (r & 1) + 8 * (r >> 1);
-          const uint16_t* src = v_head + __shfl_sync(0xffffffffu, v_row, key) + g * 8;
-          const bool there = seen >> key & 1;
-#pragma unroll
-          for (int i = 0; i < A; ++i) {
-            const bool in = there && (g + 8 * i) * 8 < p.head_dim;
-            copy16(at + (A * 4 + r * A + i) * 512, in ? src + i * 64 : v_head, in);
-          }
-        }
-        next_page = look_up(j + 1);
-      }
-      copies_commit();
-    };
-
-    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-    float o[A * 8][4];
-#pragma unroll
-    for (int i = 0; i < A * 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-
-    int stage_in = 0, stage_out = 0;
-#pragma unroll
-    for (int s = 0; s < C::kStages - 1; ++s) {
-      issue(j0 + s, stage_in);
-      ++stage_in;
+      for (int i = 0; i < A * 4; ++i) o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.f;
     }
-    for (int j = j0; j < j1; ++j) {
-      issue(j + C::kStages - 1, stage_in);
-      if (++stage_in == C::kStages) stage_in = 0;
-      copies_wait<C::kStages - 1>();
-      __syncwarp();  // the words of seen keys are another lane's
-      const uint32_t at = queue + stage_out * C::kStageBytes;
-      const uint32_t seen = s_seen[warp][stage_out];
-      if (++stage_out == C::kStages) stage_out = 0;
+
+    for (int j = seg.j0 + warp; j < seg.j1; j += W) {
+      warp_wait(&bars[stage], phase, ctl, kWaitPaged + 1);
+      const uint32_t at = queue + stage * C::kStageBytes;
+      const uint32_t seen = seen_of[0];
       const int key0 = first_key(j);
-      if (key0 >= end_all) continue;  // past the end of the sequence
-      // ---- scores of keys key0 + 2 t4, + 1 (s[0]) and + 8, + 9 (s[1])
-      float s[2][4];
+      // ---- scores, transposed: of keys key0 + g and + 8 (s[2], s[3]) for rows 2 t4 and 2 t4 + 1 of each tile
+      float s[NT][4], s2[NT][4];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+      for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = s2[n][0] = s2[n][1] = s2[n][2] = s2[n][3] = 0.f;
 #pragma unroll
       for (int i = 0; i < A * 2; ++i) {
+        const uint4 w0 = lds16(at + k_at[i & 1] + (i >> 1) * C::kPart), w1 = lds16(at + k_at[i & 1] + (i >> 1) * C::kPart + 1024);
+        const uint32_t a0[4] = {w0.x, w1.x, w0.y, w1.y}, a1[4] = {w0.z, w1.z, w0.w, w1.w};
+        uint4 b[NT];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint4 w = lds16(at + (half * (A * 2) + i) * 512);
-          mma16816<BF16>(s[half], qf[2 * i], w.x, w.y);
-          mma16816<BF16>(s[half], qf[2 * i + 1], w.z, w.w);
+        for (int n = 0; n < NT; ++n) {
+          if constexpr (C::kQInRegs) b[n] = qf[n * (A * 2) + i];
+          else b[n] = lds16(q_smem + (n * (A * 2) + i) * 512);
+        }
+        // Neighbouring products have different sums.
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma16816<BF16>(s[n], a0, b[n].x, b[n].y);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma16816<BF16>(s2[n], a1, b[n].z, b[n].w);
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] += s2[n][e];
+      const bool uneven = key0 + 16 > same_hi || key0 < same_lo;  // rows of the call see different keys of these
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        if (p.softcap > 0.f) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[n][e] = cap_l2 * tanhf(s[n][e] * inv_cap);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[n][e] *= p.scale_log2;
         }
       }
-      if (p.softcap > 0.f) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[i][e] = cap_l2 * tanhf(s[i][e] * inv_cap);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[i][e] *= p.scale_log2;
-      }
-      const bool uneven = key0 + 16 > same_hi || key0 < same_lo;  // rows of the call see different keys of these
       if (uneven || seen != 0xffffu) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int n = 2 * t4 + (e & 1) + 8 * i, key = key0 + n;
-            if (!(seen >> n & 1) || key >= ((e & 2) ? hi1 : hi0) || key < ((e & 2) ? lo1 : lo0)) s[i][e] = -INFINITY;
+            const int k = g + 8 * (e >> 1), q = p.group.div(row0 + 8 * n + 2 * t4 + (e & 1));
+            if (!(seen >> k & 1) || key0 + k >= to(q) || key0 + k < from(q)) s[n][e] = -INFINITY;
           }
       }
       if (p.scores != nullptr) {
-        float* to = p.scores + ((static_cast<int64_t>(seg.b) * p.heads_k + seg.hk) * p.rows + r0) * p.score_stride + key0 + 2 * t4;
+        float* out = p.scores + ((static_cast<int64_t>(seg.b) * p.heads_k + seg.hk) * p.rows + row0 + 2 * t4) * p.score_stride + key0 + g;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (r0 < p.rows) __stcg(reinterpret_cast<float2*>(to + 8 * i), make_float2(s[i][0], s[i][1]));
-          if (r1 < p.rows) __stcg(reinterpret_cast<float2*>(to + 8 * p.score_stride + 8 * i), make_float2(s[i][2], s[i][3]));
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (8 * n + 2 * t4 + (e & 1) < rows) __stcg(out + (8 * n + (e & 1)) * p.score_stride + 8 * (e >> 1), s[n][e]);
+      }
+      // ---- row maxima: the running ones hold until some score exceeds them
+      bool more = false;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) more = more || fmaxf(s[n][e], s[n][2 + e]) > m[n][e];
+      if (__any_sync(0xffffffffu, more)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float x = fmaxf(s[n][e], s[n][2 + e]);
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+            x = fmaxf(fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16)), m[n][e]);
+            const float f = part_scale(m[n][e], x);
+            m[n][e] = x;
+            l[n][e] *= f;
+#pragma unroll
+            for (int i = 0; i < A * 4; ++i) {
+              o[i][n][e] *= f;
+              o[i][n][2 + e] *= f;
+            }
+          }
+      }
+      uint32_t p_hi[NT][2], p_lo[NT][2];  // B fragments: keys 2 t4, + 1 (and + 8, + 9) of row g
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const float b0 = m[n][0] == -INFINITY ? 0.f : m[n][0], b1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float e0 = ex2(s[n][2 * h] - b0), e1 = ex2(s[n][2 * h + 1] - b1);
+          l[n][0] += e0;
+          l[n][1] += e1;
+          uint32_t hi, lo;
+          split2<BF16>(e0, e1, hi, lo);
+          p_hi[n][h] = transposed(hi);
+          p_lo[n][h] = transposed(lo);
         }
       }
-      // ---- row maxima over the four lanes of a row, rescale
-      float x0 = fmaxf(max3(s[0][0], s[0][1], s[1][0]), s[1][1]);
-      float x1 = fmaxf(max3(s[0][2], s[0][3], s[1][2]), s[1][3]);
-#pragma unroll
-      for (int d = 1; d < 4; d <<= 1) {
-        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
-        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
-      }
-      const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
-      if (__any_sync(0xffffffffu, n0 > m0 || n1 > m1)) {
-        const float a0 = part_scale(m0, n0), a1 = part_scale(m1, n1);
-        l0 *= a0;
-        l1 *= a1;
-#pragma unroll
-        for (int i = 0; i < A * 8; ++i) {
-          o[i][0] *= a0;
-          o[i][1] *= a0;
-          o[i][2] *= a1;
-          o[i][3] *= a1;
-        }
-        m0 = n0;
-        m1 = n1;
-      }
-      const float b0 = m0 == -INFINITY ? 0.f : m0, b1 = m1 == -INFINITY ? 0.f : m1;
-      uint32_t hi_p[4], lo_p[4];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float e0 = ex2(s[i][0] - b0), e1 = ex2(s[i][1] - b0), e2 = ex2(s[i][2] - b1), e3 = ex2(s[i][3] - b1);
-        l0 += e0 + e1;
-        l1 += e2 + e3;
-        split2<BF16>(e0, e1, hi_p[2 * i], lo_p[2 * i]);
-        split2<BF16>(e2, e3, hi_p[2 * i + 1], lo_p[2 * i + 1]);
-      }
-      // ---- O += P V: output tile 8 i + j holds columns 64 i + 8 n + j for n = 0..7
+      // ---- O^T += V^T P^T: row g of output tile 4 i + h is column 64 i + 8 g + 2 h, row g + 8 the one behind it
+      auto value = [&](int r, int i) { return lds16(at + v_at[r & 1] + (r >> 1) * 1024 + i * C::kPart); };  // of key 2 t4 + (r & 1) + 8 (r / 2)
       bool apart = false;
       if (uneven && p.seqlen_q > 1) {
         bool odd = false;
 #pragma unroll
         for (int i = 0; i < A * 4; ++i) {
-          const uint4 w = lds16(at + (A * 4 + i) * 512);
-          odd = odd || not_finite<BF16>(w.x) || not_finite<BF16>(w.y) || not_finite<BF16>(w.z) || not_finite<BF16>(w.w);
+          const uint4 w = value(i & 3, i >> 2);
+          if (seen >> (2 * t4 + (i & 1) + 8 * (i >> 1 & 1)) & 1) odd = odd || not_finite<BF16>(w.x) || not_finite<BF16>(w.y) || not_finite<BF16>(w.z) || not_finite<BF16>(w.w);
         }
         apart = __any_sync(0xffffffffu, odd);
       }
-      auto columns = [&](int i, const uint4 (&w)[4], int jj, uint32_t& c0, uint32_t& c1) {
-        const uint32_t pick = jj & 1 ? 0x7632u : 0x5410u;
-        auto word = [&](const uint4& v) { return jj < 2 ? v.x : jj < 4 ? v.y : jj < 6 ? v.z : v.w; };
-        c0 = __byte_perm(word(w[0]), word(w[1]), pick);
-        c1 = __byte_perm(word(w[2]), word(w[3]), pick);
-      };
-      if (!apart) {
+      // Calls f(output tile, its A fragment); `keep` masks the keys 2 t4 and 2 t4 + 1, and those 8 behind, by halves of a word.
+      auto values = [&](uint32_t keep0, uint32_t keep1, auto&& f) {
 #pragma unroll
         for (int i = 0; i < A; ++i) {
           uint4 w[4];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) w[r] = lds16(at + (A * 4 + r * A + i) * 512);
+          for (int r = 0; r < 4; ++r) w[r] = value(r, i);
 #pragma unroll
-          for (int jj = 0; jj < 8; ++jj) {
-            uint32_t c0, c1;
-            columns(i, w, jj, c0, c1);
-            mma16816<BF16>(o[8 * i + jj], hi_p, c0, c1);
-            mma16816<BF16>(o[8 * i + jj], lo_p, c0, c1);
+          for (int h = 0; h < 4; ++h) {
+            auto word = [&](const uint4& v) { return h == 0 ? v.x : h == 1 ? v.y : h == 2 ? v.z : v.w; };
+            const uint32_t a[4] = {__byte_perm(word(w[0]), word(w[1]), 0x5410) & keep0, __byte_perm(word(w[0]), word(w[1]), 0x7632) & keep0,
+                                   __byte_perm(word(w[2]), word(w[3]), 0x5410) & keep1, __byte_perm(word(w[2]), word(w[3]), 0x7632) & keep1};
+            f(4 * i + h, a);
           }
         }
+      };
+      auto add_all = [&](int i, const uint32_t (&a)[4]) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma16816<BF16>(o[i][n], a, p_hi[n][0], p_hi[n][1]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma16816<BF16>(o[i][n], a, p_lo[n][0], p_lo[n][1]);
+      };
+      // What was not copied, or lies under a mask of all rows, may be anything: it counts as zero.
+      auto halves = [](uint32_t bits) { return (bits & 1 ? 0xffffu : 0u) | (bits & 2 ? 0xffff0000u : 0u); };
+      if (seen == 0xffffu && !apart) {
+        values(0xffffffffu, 0xffffffffu, add_all);
+      } else if (!apart) {
+        values(halves(seen >> (2 * t4)), halves(seen >> (2 * t4 + 8)), add_all);
       } else {
         // One query at a time, with the values that it does not see at zero, into the rows of that query alone.
-        for (int q = p.group.div(seg.rt * 16); q <= p.group.div(seg.rt * 16 + rows - 1); ++q) {
-          const int to = seg.length - p.seqlen_q + q + 1, from = p.window < 0 ? 0 : to - 1 - p.window;
-          uint32_t keep[2];  // of the keys 2 t4 and 2 t4 + 1, and of those 8 behind, by halves of a word
+        for (int q = p.group.div(row0); q <= p.group.div(row0 + rows - 1); ++q) {
+          const uint32_t sees = seen & bit_range(from(q) - key0, to(q) - key0);
+          values(halves(sees >> (2 * t4)), halves(sees >> (2 * t4 + 8)), [&](int i, const uint32_t (&a)[4]) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int key = key0 + 2 * t4 + 8 * h;
-            keep[h] = (key >= from && key < to ? 0xffffu : 0u) | (key + 1 >= from && key + 1 < to ? 0xffff0000u : 0u);
-          }
+            for (int n = 0; n < NT; ++n) {
+              float c[4] = {0.f, 0.f, 0.f, 0.f};
+              mma16816<BF16>(c, a, p_hi[n][0], p_hi[n][1]);
+              mma16816<BF16>(c, a, p_lo[n][0], p_lo[n][1]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (p.group.div(row0 + 8 * n + 2 * t4 + (e & 1)) == q) o[i][n][e] += c[e];
+            }
+          });
+        }
+      }
+      // ---- the stage is free: the next tile's copies
+#pragma unroll
+      for (int i = 0; i + 1 < kStages; ++i) seen_of[i] = seen_of[i + 1];
+      __syncwarp();
+      if (j + kStages * W < seg.j1) {
+        seen_of[kStages - 1] = issue(j + kStages * W, next_page, stage);
+        next_page = look_up(j + (kStages + 1) * W);
+      }
+      if (++stage == kStages) {
+        stage = 0;
+        phase ^= 1;
+      }
+    }
+
+    // ---- the next unit's copies start, then the warps' parts become one, 8 rows at a time
+    const Segment done = seg;
+    const bool whole = done.j0 == 0 && done.j1 == done.tiles;
+    const int64_t next = done.start + done.j1;
+    more = next < hi;
+    if (more) {
+      seg.start += seg.tiles;
+      if (++seg.unit == units_per_seq) {
+        seg.unit = 0;
+        if (++seg.b >= p.batch) more = false;
+        else {
+          seg.length = length_of(seg.b);
+          open_sequence();
+        }
+      }
+      if (more) {
+        open_unit(next);
+        fill();
+      }
+    }
+    float* const slot = p.partials + (2 * static_cast<int64_t>(blockIdx.x) + (done.j0 == 0 ? 1 : 0)) * kSlot;
+    float* const parts = reinterpret_cast<float*>(smem + C::kPartOff);  // [warp][8 rows][D + 4]
+    const int warps = min(W, done.j1 - done.j0);  // those that had a tile
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      if (8 * n >= rows) break;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float x = l[n][e];
+        x += __shfl_xor_sync(0xffffffffu, x, 4);
+        x += __shfl_xor_sync(0xffffffffu, x, 8);
+        x += __shfl_xor_sync(0xffffffffu, x, 16);
+        const int r = 2 * t4 + e;
+        if (g == 0) {
+          s_m[warp][r] = m[n][e];
+          s_l[warp][r] = x;
+        }
+        if (warp < warps && 8 * n + r < rows) {
+          float* row = parts + (warp * 8 + r) * C::kRowFloats + 8 * g;
 #pragma unroll
           for (int i = 0; i < A; ++i) {
-            uint4 w[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) w[r] = lds16(at + (A * 4 + r * A + i) * 512);
-#pragma unroll
-            for (int jj = 0; jj < 8; ++jj) {
-              uint32_t c0, c1;
-              columns(i, w, jj, c0, c1);
-              float c[4] = {0.f, 0.f, 0.f, 0.f};
-              mma16816<BF16>(c, hi_p, c0 & keep[0], c1 & keep[1]);
-              mma16816<BF16>(c, lo_p, c0 & keep[0], c1 & keep[1]);
-              if (q0 == q) o[8 * i + jj][0] += c[0], o[8 * i + jj][1] += c[1];
-              if (q1 == q) o[8 * i + jj][2] += c[2], o[8 * i + jj][3] += c[3];
-            }
+            *reinterpret_cast<float4*>(row + i * 64) = make_float4(o[4 * i][n][e], o[4 * i][n][2 + e], o[4 * i + 1][n][e], o[4 * i + 1][n][2 + e]);
+            *reinterpret_cast<float4*>(row + i * 64 + 4) = make_float4(o[4 * i + 2][n][e], o[4 * i + 2][n][2 + e], o[4 * i + 3][n][e], o[4 * i + 3][n][2 + e]);
           }
         }
       }
-    }
-    copies_wait<0>();
-
-    // ---- the warps' parts become one
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-    if (t4 == 0) {
-      s_m[warp][g] = m0;
-      s_m[warp][g + 8] = m1;
-      s_l[warp][g] = l0;
-      s_l[warp][g + 8] = l1;
-    }
-    float* const parts = reinterpret_cast<float*>(smem);  // [warp][row][D + 4]; a warp's is inside its own queue
-    constexpr int kWarpFloats = C::kStages * C::kStageBytes / 4;
-    {
-      float* row0 = parts + warp * kWarpFloats + g * C::kRowFloats + 16 * t4;
-      float* row1 = row0 + 8 * C::kRowFloats;
-#pragma unroll
-      for (int i = 0; i < A; ++i)
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {  // four columns: n = 2 t4 + h / 2, j = 4 (h % 2) ...
-          const int jj = 8 * i + 4 * (h & 1), e = h >> 1;
-          if (g < rows) *reinterpret_cast<float4*>(row0 + i * 64 + h * 4) = make_float4(o[jj][e], o[jj + 1][e], o[jj + 2][e], o[jj + 3][e]);
-          if (g + 8 < rows) *reinterpret_cast<float4*>(row1 + i * 64 + h * 4) = make_float4(o[jj][2 + e], o[jj + 1][2 + e], o[jj + 2][2 + e], o[jj + 3][2 + e]);
+      __syncthreads();
+      for (int i = tid; i < min(8, rows - 8 * n) * (D / 4); i += C::kThreads) {
+        const int r = i / (D / 4), col = i % (D / 4) * 4;
+        float top = -INFINITY;
+        for (int w = 0; w < warps; ++w) top = fmaxf(top, s_m[w][r]);
+        float total = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int w = 0; w < warps; ++w) {
+          const float f = part_scale(s_m[w][r], top);
+          const float4 v = *reinterpret_cast<const float4*>(parts + (w * 8 + r) * C::kRowFloats + col);
+          total += f * s_l[w][r];
+          acc.x += f * v.x;
+          acc.y += f * v.y;
+          acc.z += f * v.z;
+          acc.w += f * v.w;
         }
-    }
-    __syncthreads();
-    const bool whole = j0 == 0 && j1 == seg.tiles;
-    constexpr int kPart = kPagedRows * (D + 2);
-    float* part = p.partials + (2 * static_cast<int64_t>(blockIdx.x) + (j0 == 0 ? 1 : 0)) * kPart;
-    auto store_out = [&](int r, int col, float4 v) {
-      if (col >= p.head_dim) return;
-      const int row = seg.rt * 16 + r, q = p.group.div(row), h = seg.hk * group + row - q * group;
-      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.o) + seg.b * p.os.outer + q * p.os.row + h * p.os.head + col) =
-          make_uint2(pack2<BF16>(v.x, v.y), pack2<BF16>(v.z, v.w));
-    };
-    // A row's end: LSE (+inf for a row that saw no key), and what turns scores into weights.
-    auto store_stats = [&](int r, float m, float l) {
-      const int row = seg.rt * 16 + r, q = p.group.div(row), h = seg.hk * group + row - q * group;
-      p.lse[(static_cast<int64_t>(seg.b) * p.heads + h) * p.seqlen_q + q] = l == 0.f ? INFINITY : (m + log2f(l)) * kLn2;
-      if (p.stats != nullptr)
-        __stcg(p.stats + (static_cast<int64_t>(seg.b) * p.heads_k + seg.hk) * p.rows + row, make_float2(m, l == 0.f ? 0.f : 1.f / l));
-    };
-    for (int i = tid; i < rows * (D / 4); i += C::kThreads) {
-      const int r = i / (D / 4), col = i % (D / 4) * 4;
-      float m = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < W; ++w) m = fmaxf(m, s_m[w][r]);
-      float l = 0.f;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < W; ++w) {
-        const float f = part_scale(s_m[w][r], m);
-        const float4 v = *reinterpret_cast<const float4*>(parts + w * kWarpFloats + r * C::kRowFloats + col);
-        l += f * s_l[w][r];
-        acc.x += f * v.x;
-        acc.y += f * v.y;
-        acc.z += f * v.z;
-        acc.w += f * v.w;
-      }
-      if (whole) {
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        store_out(r, col, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
-        if (col == 0) store_stats(r, m, l);
-      } else {
-        __stcg(reinterpret_cast<float4*>(part + r * D + col), acc);
-        if (col == 0) {
-          __stcg(part + kPagedRows * D + r, m);
-          __stcg(part + kPagedRows * D + kPagedRows + r, l);
+        if (whole) {
+          store_row(done.b, done.hk, row0 + 8 * n + r, col, acc, top, total);
+        } else {
+          __stcg(reinterpret_cast<float4*>(slot + (8 * n + r) * D + col), acc);
+          if (col == 0) {
+            __stcg(slot + R * D + 8 * n + r, top);
+            __stcg(slot + R * D + R + 8 * n + r, total);
+          }
         }
       }
+      __syncthreads();
     }
-    __syncthreads();  // the parts are in memory; the queue is free again
     if (!whole) {
-      // CTAs whose shares touch this unit: the owners of its first and its last tile. Slot 2 c holds a segment that began before
-      // CTA c's share, 2 c + 1 one that began in it.
-      const int c_first = share_owner(seg_start, n_tiles, ctas);
-      const int c_last = share_owner(seg_start + seg.tiles - 1, n_tiles, ctas);
-      auto slot_of = [&](int c) { return 2 * c + (c == c_first ? 1 : 0); };
-      if (warp == 0) {
-        // One flag per part, set to the launch's number once the part is in memory: a flag left over from another launch, or
-        // from other use of the memory, is not set. Whoever sees all of a unit's flags set merges: the last to set one does
-        // (store, fence, load); two may, and then both write the same bits.
+      // One flag per part, set to the launch's number once the part is in memory: a flag left over from another launch, or from
+      // other use of the memory, is not set. All threads' stores come before the barrier; this thread's fence behind it makes them
+      // the flag's predecessors. Slot 2 c holds a segment that began before CTA c's share, 2 c + 1 one that began in it.
+      if (tid == 0) {
+        s_pending[n_pending] = Pending{done.b, done.hk, done.rt, done.tiles, done.start};
+        asm volatile("fence.acq_rel.gpu;" ::: "memory");
+        *const_cast<volatile unsigned long long*>(p.flags + 2 * blockIdx.x + (done.j0 == 0 ? 1 : 0)) = p.launch_tag;
+      }
+      ++n_pending;
+    }
+  }
+
+  // ---- units whose last part is done: whoever sees all of a unit's flags set adds the parts up. The last to set one does (store,
+  // fence, load); others may, and then all write the same bits.
+  if (n_pending > 0) {
+    if (warp == 0) {
+      __syncwarp();
+      asm volatile("fence.sc.gpu;" ::: "memory");
+      for (int u = 0; u < n_pending; ++u) {
+        const int c_first = share_owner(s_pending[u].start, n_tiles, ctas);
+        const int c_last = share_owner(s_pending[u].start + s_pending[u].tiles - 1, n_tiles, ctas);
         volatile unsigned long long* flags = p.flags;
-        if (lane == 0) {
-          asm volatile("fence.acq_rel.gpu;" ::: "memory");
-          flags[slot_of(blockIdx.x)] = p.launch_tag;
-        }
-        __syncwarp();
-        asm volatile("fence.sc.gpu;" ::: "memory");
         bool all = true;
-        for (int c = c_first + lane; c <= c_last; c += 32) all = all && flags[slot_of(c)] == p.launch_tag;
+        for (int c = c_first + lane; c <= c_last; c += 32) all = all && flags[2 * c + (c == c_first ? 1 : 0)] == p.launch_tag;
         all = __all_sync(0xffffffffu, all);
         asm volatile("fence.acq_rel.gpu;" ::: "memory");
         if (all) {
           // A replayed graph launches with the same number: it has to find the flags clear.
-          for (int c = c_first + lane; c <= c_last; c += 32) flags[slot_of(c)] = 0;
+          for (int c = c_first + lane; c <= c_last; c += 32) flags[2 * c + (c == c_first ? 1 : 0)] = 0;
         }
-        if (lane == 0) s_last = all ? 1 : 0;
-      }
-      __syncthreads();
-      if (s_last) {
-        const int n_parts = c_last - c_first + 1;
-        for (int i = tid; i < rows * (D / 4); i += C::kThreads) {
-          const int r = i / (D / 4), col = i % (D / 4) * 4;
-          float m = -INFINITY, l = 0.f;
-          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-          constexpr int kBatch = 8;
-          for (int c0 = 0; c0 < n_parts; c0 += kBatch) {
-            float4 v[kBatch];
-            float pm[kBatch], pl[kBatch];
-#pragma unroll
-            for (int e = 0; e < kBatch; ++e) {
-              pm[e] = -INFINITY;
-              if (c0 + e < n_parts) {
-                const float* from = p.partials + static_cast<int64_t>(slot_of(c_first + c0 + e)) * kPart;
-                v[e] = __ldcg(reinterpret_cast<const float4*>(from + r * D + col));
-                pm[e] = __ldcg(from + kPagedRows * D + r);
-                pl[e] = __ldcg(from + kPagedRows * D + kPagedRows + r);
-              }
-            }
-            float top = m;
-#pragma unroll
-            for (int e = 0; e < kBatch; ++e) top = fmaxf(top, pm[e]);
-            const float f = part_scale(m, top);
-            l *= f;
-            acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
-            m = top;
-#pragma unroll
-            for (int e = 0; e < kBatch; ++e)
-              if (c0 + e < n_parts) {
-                const float f = part_scale(pm[e], m);
-                l += f * pl[e];
-                acc.x += f * v[e].x;
-                acc.y += f * v[e].y;
-                acc.z += f * v[e].z;
-                acc.w += f * v[e].w;
-              }
-          }
-          const float inv = l == 0.f ? 0.f : 1.f / l;
-          store_out(r, col, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
-          if (col == 0) store_stats(r, m, l);
-        }
+        if (lane == 0) s_parts[u] = make_int2(c_first, all ? c_last - c_first + 1 : 0);
       }
     }
-    // ---- the next unit
-    x = seg_start + j1;
-    if (j1 == seg.tiles) {
-      seg_start += seg.tiles;
-      if (++unit == units_per_seq) {
-        unit = 0;
-        if (++seg.b >= p.batch) break;
-        if (x < hi) open_sequence();
+    __syncthreads();
+    for (int u = 0; u < n_pending; ++u) {
+      const int c_first = s_parts[u].x, n_parts = s_parts[u].y;
+      if (n_parts == 0) continue;
+      const int row0 = s_pending[u].rt * R, rows = min(R, p.rows - row0);
+      for (int i = tid; i < rows * (D / 4); i += C::kThreads) {
+        const int r = i / (D / 4), col = i % (D / 4) * 4;
+        float top = -INFINITY, total = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        constexpr int kBatch = 10;  // parts whose loads are in flight together
+        for (int c0 = 0; c0 < n_parts; c0 += kBatch) {
+          float4 v[kBatch];
+          float pm[kBatch], pl[kBatch];
+#pragma unroll
+          for (int e = 0; e < kBatch; ++e) {
+            pm[e] = -INFINITY;
+            if (c0 + e < n_parts) {
+              const float* src = p.partials + (2 * static_cast<int64_t>(c_first + c0 + e) + (c0 + e == 0 ? 1 : 0)) * kSlot;
+              v[e] = __ldcg(reinterpret_cast<const float4*>(src + r * D + col));
+              pm[e] = __ldcg(src + R * D + r);
+              pl[e] = __ldcg(src + R * D + R + r);
+            }
+          }
+          float above = top;
+#pragma unroll
+          for (int e = 0; e < kBatch; ++e) above = fmaxf(above, pm[e]);
+          const float f = part_scale(top, above);
+          total *= f;
+          acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
+          top = above;
+#pragma unroll
+          for (int e = 0; e < kBatch; ++e)
+            if (c0 + e < n_parts) {
+              const float f = part_scale(pm[e], top);
+              total += f * pl[e];
+              acc.x += f * v[e].x;
+              acc.y += f * v[e].y;
+              acc.z += f * v[e].z;
+              acc.w += f * v[e].w;
+            }
+        }
+        store_row(s_pending[u].b, s_pending[u].hk, row0 + r, col, acc, top, total);
       }
     }
   }
+  if (s_abort) {
+    // A wait ran out: copies may still be in flight, give them about a millisecond before the memory is given back.
+    const long long t0 = clock64();
+    while (clock64() - t0 < 2000000) {
+    }
+  }
+  __syncthreads();
+  if (tid == 0) report_abort(&s_abort, p.status);
 }
 
 // mass[page][kv head][row] += sum over the query rows of exp2(score - maximum) / sum. One thread a key; the sum is in the order of
@@ -617,26 +735,41 @@ __global__ void __launch_bounds__(kMassThreads) paged_mass_kernel(const __grid_c
   }
 }
 
-template <int A, bool BF16>
+template <int A, int NT, bool BF16, bool TILED>
 cudaError_t launch_one(const PagedParams& p, int grid, cudaStream_t stream) {
-  using C = Cfg<A>;
+  using C = Cfg<A, NT>;
   static bool configured[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 0 && dev < 64 && !configured[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(fwd_paged_kernel<A, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+    cudaError_t e = cudaFuncSetAttribute(fwd_paged_kernel<A, NT, BF16, TILED>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
     if (e != cudaSuccess) return e;
     configured[dev] = true;
   }
-  return launch_grid(true, fwd_paged_kernel<A, BF16>, dim3(grid), C::kThreads, C::kSmemBytes, stream, p);
+  return launch_grid(true, fwd_paged_kernel<A, NT, BF16, TILED>, dim3(grid), C::kThreads, C::kSmemBytes, stream, p);
+}
+
+template <int A, int NT, bool BF16>
+cudaError_t pick_copies(const PagedParams& p, int grid, cudaStream_t stream) {
+  return p.tiled ? launch_one<A, NT, BF16, true>(p, grid, stream) : launch_one<A, NT, BF16, false>(p, grid, stream);
+}
+
+template <int A, bool BF16>
+cudaError_t pick_rows(const PagedParams& p, int grid, cudaStream_t stream) {
+  const int rows = paged_unit_rows(p.head_dim, p.rows);
+  if (rows == 8) return pick_copies<A, 1, BF16>(p, grid, stream);
+  if constexpr (A <= 2) {
+    if (rows == 32) return pick_copies<A, 4, BF16>(p, grid, stream);
+  }
+  return pick_copies<A, 2, BF16>(p, grid, stream);
 }
 
 template <bool BF16>
 cudaError_t pick_dim(const PagedParams& p, int grid, cudaStream_t stream) {
-  if (p.head_dim <= 64) return launch_one<1, BF16>(p, grid, stream);
-  if (p.head_dim <= 128) return launch_one<2, BF16>(p, grid, stream);
-  if (p.head_dim <= 192) return launch_one<3, BF16>(p, grid, stream);
-  return launch_one<4, BF16>(p, grid, stream);
+  if (p.head_dim <= 64) return pick_rows<1, BF16>(p, grid, stream);
+  if (p.head_dim <= 128) return pick_rows<2, BF16>(p, grid, stream);
+  if (p.head_dim <= 192) return pick_rows<3, BF16>(p, grid, stream);
+  return pick_rows<4, BF16>(p, grid, stream);
 }
 
 }  // namespace

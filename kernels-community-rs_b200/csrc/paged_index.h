@@ -71,9 +71,16 @@ FA2_BOTH int tiles_of(int length, int seqlen_q, int window, int tile) {
   const int n = end - first_seen_tile(length, seqlen_q, window, tile);
   return n > 0 ? n : 1;
 }
-// CTA c of `grid` has the tiles [share_begin(c), share_begin(c + 1)) of the list; share_owner gives the CTA of a tile.
-FA2_BOTH int64_t share_begin(int64_t c, int64_t tiles, int64_t grid) { return c * tiles / grid; }
+// CTA c of `grid` has the tiles [share_begin(c), share_begin(c + 1)) of the list; share_owner gives the CTA of a tile. Lists of
+// usual lengths get by with 32-bit divisions.
+FA2_BOTH bool share_is_small(int64_t tiles, int64_t grid) { return tiles < (1 << 24) && grid < 255; }
+FA2_BOTH int64_t share_begin(int64_t c, int64_t tiles, int64_t grid) {
+  if (share_is_small(tiles, grid)) return static_cast<uint32_t>(c) * static_cast<uint32_t>(tiles) / static_cast<uint32_t>(grid);
+  return c * tiles / grid;
+}
 FA2_BOTH int share_owner(int64_t tile, int64_t tiles, int64_t grid) {
+  if (share_is_small(tiles, grid))
+    return static_cast<int>((static_cast<uint32_t>(tile + 1) * static_cast<uint32_t>(grid) + static_cast<uint32_t>(tiles) - 1) / static_cast<uint32_t>(tiles) - 1);
   return static_cast<int>(((tile + 1) * grid + tiles - 1) / tiles - 1);
 }
 
