@@ -4,8 +4,6 @@
 #include "fa2_runtime.h"
 
 #include <algorithm>
-#include <atomic>
-#include <chrono>
 #include <climits>
 #include <cmath>
 #include <cstring>
@@ -145,8 +143,8 @@ int rotary_launch(fa2::RotaryParams* p, int dtype, bool append, bool vectors, Ru
 struct FwdPlan {
   int most_keys = 0, rows = 0, row_tiles = 0, grid = 0;
   int64_t score_stride = 0;
-  int64_t flag_bytes = 0, part_bytes = 0, stat_bytes = 0, score_bytes = 0;
-  int64_t bytes() const { return flag_bytes + part_bytes + stat_bytes + score_bytes; }
+  int64_t list_bytes = 0, part_bytes = 0, stat_bytes = 0, score_bytes = 0;
+  int64_t bytes() const { return list_bytes + part_bytes + stat_bytes + score_bytes; }
 };
 int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
 
@@ -159,7 +157,7 @@ int plan_fwd(const fa2_paged_fwd_args* a, int sm_count, FwdPlan* f) {
   f->row_tiles = (f->rows + unit_rows - 1) / unit_rows;
   const int64_t most_tiles = static_cast<int64_t>(c->batch) * c->heads_k * f->row_tiles * ((f->most_keys + static_cast<int64_t>(fa2::kPagedTile) - 1) / fa2::kPagedTile);
   f->grid = static_cast<int>(std::min<int64_t>(sm_count, (most_tiles + fa2::kPagedMinShare - 1) / fa2::kPagedMinShare));
-  f->flag_bytes = round256(2 * static_cast<int64_t>(f->grid) * 8);
+  f->list_bytes = round256(static_cast<int64_t>(f->grid) * 16);
   f->part_bytes = round256(2 * static_cast<int64_t>(f->grid) * fa2::paged_part_floats(c->head_dim, f->rows) * 4);
   if (c->attn_mass != nullptr) {
     const int64_t rows = static_cast<int64_t>(c->batch) * c->heads_k * f->rows;
@@ -302,18 +300,14 @@ int fa2_paged_fwd(const fa2_paged_fwd_args* args, void* workspace, int64_t works
   p.scale_log2 = args->softmax_scale * 1.4426950408889634f;
   p.softcap = args->softcap;
   char* at = static_cast<char*>(workspace);
-  p.flags = reinterpret_cast<unsigned long long*>(at);
-  p.partials = reinterpret_cast<float*>(at += f.flag_bytes);
+  p.shared = reinterpret_cast<int4*>(at);
+  p.partials = reinterpret_cast<float*>(at += f.list_bytes);
   if (c->attn_mass != nullptr) {
     p.stats = reinterpret_cast<float2*>(at += f.part_bytes);
     p.scores = reinterpret_cast<float*>(at += f.stat_bytes);
     p.score_stride = f.score_stride;
     p.mass = c->attn_mass;
   }
-  // The flags in the workspace are set to this number, so their old contents do not matter.
-  static std::atomic<unsigned long long> launches{static_cast<unsigned long long>(
-      std::chrono::steady_clock::now().time_since_epoch().count())};
-  p.launch_tag = (launches.fetch_add(1) + 1) | (1ull << 63);  // never the cleared value
   p.status = rt->status;
   cudaError_t e = fa2::launch_fwd_paged(p, f.grid, c->dtype == FA2_BF16, static_cast<cudaStream_t>(stream));
   if (e == cudaSuccess && p.mass != nullptr) e = fa2::launch_paged_mass(p, rt->sm_count, static_cast<cudaStream_t>(stream));

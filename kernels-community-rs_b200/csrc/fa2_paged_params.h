@@ -60,8 +60,7 @@ struct PagedParams {
   int window;
   float scale, scale_log2, softcap;
   float* partials;              // 2 slots per CTA
-  unsigned long long* flags;    // one per slot: launch_tag once the part is in memory
-  unsigned long long launch_tag;
+  int4* shared;                 // of the unit that begins in a CTA's share and ends in another: its parts (0: there is none), sequence, kv head, row tile
   float* scores;                // [batch, heads_k, rows, score_stride] in the log2 domain, or null
   int64_t score_stride;
   float2* stats;                // [batch, heads_k, rows]: row maximum (log2 domain), 1 / row sum

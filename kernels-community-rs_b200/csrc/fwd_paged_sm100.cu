@@ -8,7 +8,7 @@
 //   * The query rows of a kv head (row r = query r / group, head r % group) are the M of one product, 16 at a time.
 //   * The lengths are on the device. Every CTA, one per SM, adds up the sequences' key tiles and takes an equal share of the list
 //     of all (sequence, kv head, key tile); a share may begin and end inside a unit. A CTA leaves its part of a unit that it does
-//     not cover alone in the workspace, and whichever sees a unit's last part done adds the parts up, in the order of the keys.
+//     not cover alone in the workspace, and a second kernel, which waits beside the first, adds the parts up.
 //   * A thread's copies are its own. mma.sync takes B fragments whose k index may be permuted freely as long as A's is alike, and
 //     n is only a name; so lane (g, t) = (lane / 4, lane % 4) takes 16-byte pieces t, t + 4, ... of key g's row as two k-steps of
 //     Q K^T, and pieces g, g + 8, ... of the rows of keys 2t, 2t + 1, 2t + 8, 2t + 9 as columns of P V. Every lane therefore reads
@@ -115,11 +115,19 @@ struct Segment {
   int64_t start;       // list index of the unit's first tile
   int end_all, begin_all;  // keys outside [begin_all, end_all) are seen by no row
 };
-// A unit of which this CTA has left a part in the workspace.
-struct Pending {
-  int b, hk, rt, tiles;
-  int64_t start;
-};
+// Four columns of a row's end, and with the first of them the LSE (+inf for a row that saw no key) and what turns scores into weights.
+template <bool BF16>
+__device__ __forceinline__ void store_row(const PagedParams& p, int b, int hk, int row, int col, const float4& acc, float top, float total) {
+  const int q = p.group.div(row), group = static_cast<int>(p.group.d), h = hk * group + row - q * group;
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  if (col < p.head_dim)
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.o) + b * p.os.outer + q * p.os.row + h * p.os.head + col) =
+        make_uint2(pack2<BF16>(acc.x * inv, acc.y * inv), pack2<BF16>(acc.z * inv, acc.w * inv));
+  if (col == 0) {
+    p.lse[(static_cast<int64_t>(b) * p.heads + h) * p.seqlen_q + q] = total == 0.f ? INFINITY : (top + log2f(total)) * kLn2;
+    if (p.stats != nullptr) __stcg(p.stats + (static_cast<int64_t>(b) * p.heads_k + hk) * p.rows + row, make_float2(top, inv));
+  }
+}
 
 // TILED: pages are whole tiles, so that a tile is one TMA box for each 64 columns of K and of V. Otherwise its rows lie in two or more
 // pages, and are copied 16 bytes at a time.
@@ -132,8 +140,6 @@ __global__ void __launch_bounds__((Cfg<A, NT>::kThreads), 1) fwd_paged_kernel(co
   __shared__ int64_t s_before;        // tiles of the sequences before s_first
   __shared__ int s_first, s_length;   // ... and its length
   __shared__ float s_m[W][8], s_l[W][8];
-  __shared__ Pending s_pending[2];
-  __shared__ int2 s_parts[2];   // of a pending unit: its first CTA, and how many there are if all are done, or 0
   __shared__ int s_abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t4 = lane & 3;
@@ -163,13 +169,17 @@ __global__ void __launch_bounds__((Cfg<A, NT>::kThreads), 1) fwd_paged_kernel(co
     return cut_length(n, most);
   };
   auto list_of = [&](int length) { return static_cast<int64_t>(tiles_of(length, p.seqlen_q, p.window, kPagedTile)) * units_per_seq; };
-  // Sum over the threads up to this one, and over all.
-  auto scan = [&](int64_t x, int64_t& all) {
+  auto warp_scan = [&](int64_t x) {
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const int64_t y = __shfl_up_sync(0xffffffffu, x, d);
       if (lane >= d) x += y;
     }
+    return x;
+  };
+  // Sum over the threads up to this one, and over all.
+  auto scan = [&](int64_t x, int64_t& all) {
+    x = warp_scan(x);
     __syncthreads();
     if (lane == 31) s_sum[warp] = x;
     __syncthreads();
@@ -183,7 +193,23 @@ __global__ void __launch_bounds__((Cfg<A, NT>::kThreads), 1) fwd_paged_kernel(co
   };
   Segment seg;
   int64_t n_tiles, ctas, lo, hi;
-  {
+  // No CTA has nothing (a unit's parts are neighbours' parts), and none has less than a few tiles where there are more.
+  auto take_share = [&]() {
+    ctas = max(min((n_tiles + kPagedMinShare - 1) / kPagedMinShare, static_cast<int64_t>(gridDim.x)), static_cast<int64_t>(1));
+    lo = share_begin(blockIdx.x, n_tiles, ctas);
+    hi = share_begin(blockIdx.x + 1, n_tiles, ctas);
+  };
+  // Then the sequence that tile lo belongs to: its number of tiles before reaches lo last.
+  if (p.batch <= 32) {  // every warp for itself
+    const int length = lane < p.batch ? length_of(lane) : 0;
+    const int64_t n = lane < p.batch ? list_of(length) : 0, upto = warp_scan(n);
+    n_tiles = __shfl_sync(0xffffffffu, upto, 31);
+    take_share();
+    const uint32_t found = __ballot_sync(0xffffffffu, upto - n <= lo && lo < upto);
+    seg.b = found != 0 ? __ffs(found) - 1 : 0;
+    seg.start = __shfl_sync(0xffffffffu, upto - n, seg.b);
+    seg.length = __shfl_sync(0xffffffffu, length, seg.b);
+  } else {
     const int length = tid < p.batch ? length_of(tid) : 0;
     int64_t n = tid < p.batch ? list_of(length) : 0, all;
     int64_t upto = scan(n, all);
@@ -194,12 +220,7 @@ __global__ void __launch_bounds__((Cfg<A, NT>::kThreads), 1) fwd_paged_kernel(co
       scan(more, rest);
       n_tiles += rest;
     }
-    // No CTA has nothing (a unit's parts are neighbours' parts), and none has less than a few tiles where there are more.
-    ctas = max(min((n_tiles + kPagedMinShare - 1) / kPagedMinShare, static_cast<int64_t>(gridDim.x)), static_cast<int64_t>(1));
-    if (blockIdx.x >= ctas) return;  // no copy has been started
-    lo = share_begin(blockIdx.x, n_tiles, ctas);
-    hi = share_begin(blockIdx.x + 1, n_tiles, ctas);
-    // the sequence that tile lo belongs to: its number of tiles before reaches lo last
+    take_share();
     auto look = [&](int b, int seq_length) {
       if (upto - n <= lo && lo < upto) {
         s_first = b;
@@ -220,6 +241,10 @@ __global__ void __launch_bounds__((Cfg<A, NT>::kThreads), 1) fwd_paged_kernel(co
     seg.b = s_first;
     seg.start = s_before;
     seg.length = s_length;
+  }
+  if (blockIdx.x >= ctas) {  // no copy has been started
+    if (tid == 0) p.shared[blockIdx.x] = make_int4(0, 0, 0, 0);
+    return;
   }
   auto open_sequence = [&]() {
     seg.first = first_seen_tile(seg.length, p.seqlen_q, p.window, kPagedTile);
@@ -321,21 +346,8 @@ __global__ void __launch_bounds__((Cfg<A, NT>::kThreads), 1) fwd_paged_kernel(co
   };
   fill();
 
-  // Four columns of a row's end, and with the first of them the LSE (+inf for a row that saw no key) and what turns scores into weights.
-  auto store_row = [&](int b, int hk, int row, int col, const float4& acc, float top, float total) {
-    const int q = p.group.div(row), h = hk * group + row - q * group;
-    const float inv = total == 0.f ? 0.f : 1.f / total;
-    if (col < p.head_dim)
-      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.o) + b * p.os.outer + q * p.os.row + h * p.os.head + col) =
-          make_uint2(pack2<BF16>(acc.x * inv, acc.y * inv), pack2<BF16>(acc.z * inv, acc.w * inv));
-    if (col == 0) {
-      p.lse[(static_cast<int64_t>(b) * p.heads + h) * p.seqlen_q + q] = total == 0.f ? INFINITY : (top + log2f(total)) * kLn2;
-      if (p.stats != nullptr) __stcg(p.stats + (static_cast<int64_t>(b) * p.heads_k + hk) * p.rows + row, make_float2(top, inv));
-    }
-  };
   constexpr int kSlot = R * (D + 2);  // floats of a part in the workspace
 
-  int n_pending = 0;
   for (bool more = true; more;) {
     const int row0 = seg.rt * R;
     const int rows = min(R, p.rows - row0);
@@ -607,7 +619,7 @@ __global__ void __launch_bounds__((Cfg<A, NT>::kThreads), 1) fwd_paged_kernel(co
           acc.w += f * v.w;
         }
         if (whole) {
-          store_row(done.b, done.hk, row0 + 8 * n + r, col, acc, top, total);
+          store_row<BF16>(p, done.b, done.hk, row0 + 8 * n + r, col, acc, top, total);
         } else {
           __stcg(reinterpret_cast<float4*>(slot + (8 * n + r) * D + col), acc);
           if (col == 0) {
@@ -618,83 +630,10 @@ __global__ void __launch_bounds__((Cfg<A, NT>::kThreads), 1) fwd_paged_kernel(co
       }
       __syncthreads();
     }
-    if (!whole) {
-      // One flag per part, set to the launch's number once the part is in memory: a flag left over from another launch, or from
-      // other use of the memory, is not set. All threads' stores come before the barrier; this thread's fence behind it makes them
-      // the flag's predecessors. Slot 2 c holds a segment that began before CTA c's share, 2 c + 1 one that began in it.
-      if (tid == 0) {
-        s_pending[n_pending] = Pending{done.b, done.hk, done.rt, done.tiles, done.start};
-        asm volatile("fence.acq_rel.gpu;" ::: "memory");
-        *const_cast<volatile unsigned long long*>(p.flags + 2 * blockIdx.x + (done.j0 == 0 ? 1 : 0)) = p.launch_tag;
-      }
-      ++n_pending;
-    }
-  }
-
-  // ---- units whose last part is done: whoever sees all of a unit's flags set adds the parts up. The last to set one does (store,
-  // fence, load); others may, and then all write the same bits.
-  if (n_pending > 0) {
-    if (warp == 0) {
-      __syncwarp();
-      asm volatile("fence.sc.gpu;" ::: "memory");
-      for (int u = 0; u < n_pending; ++u) {
-        const int c_first = share_owner(s_pending[u].start, n_tiles, ctas);
-        const int c_last = share_owner(s_pending[u].start + s_pending[u].tiles - 1, n_tiles, ctas);
-        volatile unsigned long long* flags = p.flags;
-        bool all = true;
-        for (int c = c_first + lane; c <= c_last; c += 32) all = all && flags[2 * c + (c == c_first ? 1 : 0)] == p.launch_tag;
-        all = __all_sync(0xffffffffu, all);
-        asm volatile("fence.acq_rel.gpu;" ::: "memory");
-        if (all) {
-          // A replayed graph launches with the same number: it has to find the flags clear.
-          for (int c = c_first + lane; c <= c_last; c += 32) flags[2 * c + (c == c_first ? 1 : 0)] = 0;
-        }
-        if (lane == 0) s_parts[u] = make_int2(c_first, all ? c_last - c_first + 1 : 0);
-      }
-    }
-    __syncthreads();
-    for (int u = 0; u < n_pending; ++u) {
-      const int c_first = s_parts[u].x, n_parts = s_parts[u].y;
-      if (n_parts == 0) continue;
-      const int row0 = s_pending[u].rt * R, rows = min(R, p.rows - row0);
-      for (int i = tid; i < rows * (D / 4); i += C::kThreads) {
-        const int r = i / (D / 4), col = i % (D / 4) * 4;
-        float top = -INFINITY, total = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        constexpr int kBatch = 10;  // parts whose loads are in flight together
-        for (int c0 = 0; c0 < n_parts; c0 += kBatch) {
-          float4 v[kBatch];
-          float pm[kBatch], pl[kBatch];
-#pragma unroll
-          for (int e = 0; e < kBatch; ++e) {
-            pm[e] = -INFINITY;
-            if (c0 + e < n_parts) {
-              const float* src = p.partials + (2 * static_cast<int64_t>(c_first + c0 + e) + (c0 + e == 0 ? 1 : 0)) * kSlot;
-              v[e] = __ldcg(reinterpret_cast<const float4*>(src + r * D + col));
-              pm[e] = __ldcg(src + R * D + r);
-              pl[e] = __ldcg(src + R * D + R + r);
-            }
-          }
-          float above = top;
-#pragma unroll
-          for (int e = 0; e < kBatch; ++e) above = fmaxf(above, pm[e]);
-          const float f = part_scale(top, above);
-          total *= f;
-          acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
-          top = above;
-#pragma unroll
-          for (int e = 0; e < kBatch; ++e)
-            if (c0 + e < n_parts) {
-              const float f = part_scale(pm[e], top);
-              total += f * pl[e];
-              acc.x += f * v[e].x;
-              acc.y += f * v[e].y;
-              acc.z += f * v[e].z;
-              acc.w += f * v[e].w;
-            }
-        }
-        store_row(s_pending[u].b, s_pending[u].hk, row0 + r, col, acc, top, total);
-      }
+    // The unit that begins in this share and ends in another is paged_join_kernel's, and known there by this CTA.
+    if (!more && tid == 0) {
+      const int c_last = share_owner(done.start + done.tiles - 1, n_tiles, ctas);
+      p.shared[blockIdx.x] = make_int4(whole || done.j0 > 0 ? 0 : c_last - static_cast<int>(blockIdx.x) + 1, done.b, done.hk, done.rt);
     }
   }
   if (s_abort) {
@@ -705,6 +644,61 @@ __global__ void __launch_bounds__((Cfg<A, NT>::kThreads), 1) fwd_paged_kernel(co
   }
   __syncthreads();
   if (tid == 0) report_abort(&s_abort, p.status);
+}
+
+// The units that several CTAs share: block (c, y) adds up the parts of 8 rows of the one that begins in share c, in the order of the
+// keys. A kernel of its own, which starts early and waits beside the attention. (With flags in memory, by which the last CTA of a unit
+// knew itself, a call ended with two fences and two round trips to memory: B1 H32/8 Sk 8192 D128 17.3 us in place of 14.9.)
+constexpr int kJoinThreads = 128;  // its registers fit beside those of the attention
+template <bool BF16>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedParams p, int d, int unit_rows) {
+  early_wait();
+  early_trigger();
+  const int4 unit = p.shared[blockIdx.x];
+  const int n_parts = unit.x;
+  if (n_parts == 0) return;
+  const int row0 = unit.w * unit_rows + blockIdx.y * 8, rows = min(8, min(unit_rows - static_cast<int>(blockIdx.y) * 8, p.rows - row0));
+  const int64_t slot = static_cast<int64_t>(unit_rows) * (d + 2);
+  // Slot 2 c holds a segment that began before CTA c's share, 2 c + 1 one that began in it: the first part.
+  const float* first = p.partials + (2 * static_cast<int64_t>(blockIdx.x) + 1) * slot;
+  for (int i = threadIdx.x; i < rows * (d / 4); i += kJoinThreads) {
+    const int r = blockIdx.y * 8 + i / (d / 4), col = i % (d / 4) * 4;
+    float top = -INFINITY, total = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    constexpr int kBatch = 10;  // parts whose loads are in flight together
+    for (int c0 = 0; c0 < n_parts; c0 += kBatch) {
+      float4 v[kBatch];
+      float pm[kBatch], pl[kBatch];
+#pragma unroll
+      for (int e = 0; e < kBatch; ++e) {
+        pm[e] = -INFINITY;
+        if (c0 + e < n_parts) {
+          const float* src = first + (c0 + e == 0 ? 0 : 2 * (c0 + e) - 1) * slot;
+          v[e] = __ldcg(reinterpret_cast<const float4*>(src + r * d + col));
+          pm[e] = __ldcg(src + unit_rows * d + r);
+          pl[e] = __ldcg(src + unit_rows * d + unit_rows + r);
+        }
+      }
+      float above = top;
+#pragma unroll
+      for (int e = 0; e < kBatch; ++e) above = fmaxf(above, pm[e]);
+      const float f = part_scale(top, above);
+      total *= f;
+      acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
+      top = above;
+#pragma unroll
+      for (int e = 0; e < kBatch; ++e)
+        if (c0 + e < n_parts) {
+          const float g = part_scale(pm[e], top);
+          total += g * pl[e];
+          acc.x += g * v[e].x;
+          acc.y += g * v[e].y;
+          acc.z += g * v[e].z;
+          acc.w += g * v[e].w;
+        }
+    }
+    store_row<BF16>(p, unit.y, unit.z, unit.w * unit_rows + r, col, acc, top, total);
+  }
 }
 
 // mass[page][kv head][row] += sum over the query rows of exp2(score - maximum) / sum. One thread a key; the sum is in the order of
@@ -776,7 +770,12 @@ cudaError_t pick_dim(const PagedParams& p, int grid, cudaStream_t stream) {
 
 cudaError_t launch_fwd_paged(const PagedParams& p, int grid, bool bf16, cudaStream_t stream) {
   if (p.rows <= 0 || p.rows > kPagedMaxRows || p.head_dim <= 0 || p.head_dim > 256 || grid <= 0) return cudaErrorInvalidValue;
-  return bf16 ? pick_dim<true>(p, grid, stream) : pick_dim<false>(p, grid, stream);
+  const cudaError_t e = bf16 ? pick_dim<true>(p, grid, stream) : pick_dim<false>(p, grid, stream);
+  if (e != cudaSuccess) return e;
+  const int d = (p.head_dim + 63) / 64 * 64, unit_rows = paged_unit_rows(p.head_dim, p.rows);
+  const dim3 blocks(grid, (unit_rows + 7) / 8);
+  if (bf16) return launch_grid(true, paged_join_kernel<true>, blocks, kJoinThreads, 0, stream, p, d, unit_rows);
+  return launch_grid(true, paged_join_kernel<false>, blocks, kJoinThreads, 0, stream, p, d, unit_rows);
 }
 
 cudaError_t launch_paged_mass(const PagedParams& p, int sm_count, cudaStream_t stream) {
