@@ -100,7 +100,7 @@ int get_runtime(int device, Runtime** out) {
 // box is one 128-byte swizzle line wide and `box_rows` rows tall.
 int make_map(CUtensorMap* m, const void* ptr, int dtype, int esize, int64_t d, int64_t heads, int64_t rows,
              int64_t batch, int64_t head_stride, int64_t row_stride, int64_t batch_stride, int box_inner, int box_rows,
-             const char* name) {
+             const char* name, bool wide) {
   const int64_t inner_bytes = d * esize;
   cuuint64_t dims[4] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(rows),
                         static_cast<cuuint64_t>(batch)};
@@ -115,7 +115,7 @@ int make_map(CUtensorMap* m, const void* ptr, int dtype, int esize, int64_t d, i
                            : dtype == FA2_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   CUresult r = g_encode(m, dt, 4, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_SWIZZLE_128B, wide ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(FA2_E_VALUE, "cannot build a TMA descriptor for %s (CUresult %d)", name, (int)r);
   return FA2_OK;

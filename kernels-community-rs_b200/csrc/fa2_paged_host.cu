@@ -278,11 +278,12 @@ int fa2_paged_fwd(const fa2_paged_fwd_args* args, void* workspace, int64_t works
   p.table = table_of(c);
   p.tiled = c->page_size % fa2::kPagedTile == 0;
   if (p.tiled) {
+    const bool wide = c->head_dim * 2 % 256 == 0;
     if ((rc = fa2::make_map(&p.tm_k, c->k, c->dtype, 2, c->head_dim, c->heads_k, c->page_size, c->num_pages, c->k_stride[2], c->k_stride[1],
-                            c->k_stride[0], 64, fa2::kPagedTile, "k")) != FA2_OK)
+                            c->k_stride[0], 64, fa2::kPagedTile, "k", wide)) != FA2_OK)
       return rc;
     if ((rc = fa2::make_map(&p.tm_v, c->v, c->dtype, 2, c->head_dim, c->heads_k, c->page_size, c->num_pages, c->v_stride[2], c->v_stride[1],
-                            c->v_stride[0], 64, fa2::kPagedTile, "v")) != FA2_OK)
+                            c->v_stride[0], 64, fa2::kPagedTile, "v", wide)) != FA2_OK)
       return rc;
   }
   p.seqlens = c->seqlens_k;

@@ -23,9 +23,10 @@ struct Runtime {
 int get_runtime(int device, Runtime** out);
 
 // A tensor map over [batch][rows][heads][D] of 16-bit (dtype 2: fp32) elements; strides in elements, boxes of box_inner columns and
-// box_rows rows, 128-byte swizzle. The runtime has to be there.
+// box_rows rows, 128-byte swizzle. `wide`: L2 fetches 256 bytes at a time, which
+// brings a neighbour's data too where a row's columns are not a multiple of that. The runtime has to be there.
 int make_map(CUtensorMap* m, const void* ptr, int dtype, int esize, int64_t d, int64_t heads, int64_t rows, int64_t batch, int64_t head_stride,
-             int64_t row_stride, int64_t batch_stride, int box_inner, int box_rows, const char* name);
+             int64_t row_stride, int64_t batch_stride, int box_inner, int box_rows, const char* name, bool wide = true);
 
 // Makes the device that owns `ptr` current for the lifetime of the object and restores the caller's
 // device afterwards, as the reference binds the context of q before every launch

@@ -283,18 +283,21 @@ __global__ void __launch_bounds__((Cfg<A, NT>::kThreads), 1) fwd_paged_kernel(co
 
   // ---- copies of 16 keys of the present segment
   auto first_key = [&](int j) { return (seg.first + j) * kPagedTile; };
-  // The page of a tile (TILED), or of key `lane % 16` of it; -1: there is none, or no row sees it.
+  // The table's entry for a tile (TILED), or for key `lane % 16` of it. It is looked at when it is used: a
+  // step later, so that nothing waits for it.
   auto look_up = [&](int j) {
     const int key = first_key(j) + (TILED ? 0 : lane & 15);
     if (j >= seg.j1 || key >= seg.end_all || (!TILED && key < seg.begin_all)) return -1;
-    const int page = p.table.pages[seg.b * p.table.stride + p.table.page_size.div(key)];
-    if (static_cast<uint32_t>(page) < static_cast<uint32_t>(p.table.num_pages)) return page;
-    if (p.status != nullptr) atomicCAS(p.status, 0, static_cast<int>(kPagedBadPage));
-    return -1;
+    return p.table.pages[seg.b * p.table.stride + p.table.page_size.div(key)];
   };
   // Starts the copies of tile j into a stage that every lane has read, and returns a bit for each of its keys that some row sees.
   auto issue = [&](int j, int page, int to_stage) {
     const int key0 = first_key(j);
+    if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(p.table.num_pages)) {
+      const int key = key0 + (TILED ? 0 : lane & 15);
+      if (key < seg.end_all && key >= (TILED ? 0 : seg.begin_all) && p.status != nullptr) atomicCAS(p.status, 0, static_cast<int>(kPagedBadPage));
+      page = -1;
+    }
     const uint32_t at = queue + to_stage * C::kStageBytes;
     uint32_t seen;
     if constexpr (TILED) {
@@ -393,9 +396,10 @@ __global__ void __launch_bounds__((Cfg<A, NT>::kThreads), 1) fwd_paged_kernel(co
       const uint32_t seen = seen_of[0];
       const int key0 = first_key(j);
       // ---- scores, transposed: of keys key0 + g and + 8 (s[2], s[3]) for rows 2 t4 and 2 t4 + 1 of each tile
-      float s[NT][4], s2[NT][4];
+      constexpr int kSums = NT == 1 ? 2 : NT;  // chains of products: one alone would be waited for at each step
+      float s[kSums][4];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = s2[n][0] = s2[n][1] = s2[n][2] = s2[n][3] = 0.f;
+      for (int n = 0; n < kSums; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
 #pragma unroll
       for (int i = 0; i < A * 2; ++i) {
         const uint4 w0 = lds16(at + k_at[i & 1] + (i >> 1) * C::kPart), w1 = lds16(at + k_at[i & 1] + (i >> 1) * C::kPart + 1024);
@@ -410,12 +414,12 @@ __global__ void __launch_bounds__((Cfg<A, NT>::kThreads), 1) fwd_paged_kernel(co
 #pragma unroll
         for (int n = 0; n < NT; ++n) mma16816<BF16>(s[n], a0, b[n].x, b[n].y);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma16816<BF16>(s2[n], a1, b[n].z, b[n].w);
+        for (int n = 0; n < NT; ++n) mma16816<BF16>(s[NT == 1 ? 1 : n], a1, b[n].z, b[n].w);
       }
+      if constexpr (NT == 1) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[n][e] += s2[n][e];
+        for (int e = 0; e < 4; ++e) s[0][e] += s[1][e];
+      }
       const bool uneven = key0 + 16 > same_hi || key0 < same_lo;  // rows of the call see different keys of these
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
