@@ -128,11 +128,11 @@ int rotary_params(const fa2_rotary_args* a, fa2::RotaryParams* p) {
 int rotary_launch(fa2::RotaryParams* p, int dtype, bool append, bool vectors, Runtime* rt, cudaStream_t stream) {
   const int heads = p->heads + p->heads_k + (append ? p->heads_k : 0);
   p->heads_all = make_div(heads);
-  // About four 16-element items a thread of a block, fewer where the tokens would not fill the GPU.
-  const int64_t per_token = static_cast<int64_t>(heads) * p->items.d;
-  int64_t t = 1024 / per_token;
-  t = std::min<int64_t>(t, p->tokens / (2 * rt->sm_count));
-  p->tokens_per_block = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(t, 32)));
+  // A warp has a token's heads to itself where that fills the GPU with 16 warps per SM; else they are shared, down to a head a lane.
+  const int64_t fill = 16 * static_cast<int64_t>(rt->sm_count);
+  const int at_once = 32 / static_cast<int>(p->items.d);
+  p->warps_log = 0;
+  while ((static_cast<int64_t>(p->tokens) << p->warps_log) < fill && (at_once << p->warps_log) < heads && p->warps_log < 8) ++p->warps_log;
   p->status = rt->status;
   const cudaError_t e = fa2::launch_rotary(*p, dtype == FA2_BF16, append, vectors, stream);
   if (e != cudaSuccess) return fail(FA2_E_RUNTIME, "rotary launch failed: %s", cudaGetErrorString(e));

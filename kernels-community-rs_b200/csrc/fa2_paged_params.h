@@ -27,7 +27,7 @@ struct RotaryParams {
   int tokens;                   // batch * seqlen
   FastDiv seqlen, heads_all, items;  // rows per batch entry; heads of q, k (and v); 16-element items of a head
   int heads, heads_k, head_dim, pairs;
-  int tokens_per_block;
+  int warps_log;                // 2^warps_log warps share the heads of a token
   const void* positions;
   int64_t pos_axis, pos_batch, pos_row;
   int positions64;

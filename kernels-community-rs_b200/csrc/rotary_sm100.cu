@@ -4,10 +4,9 @@
 //
 // for the pairs (x0, x1) of a head's first elements; the others are copied. The gradient is the turn by -a.
 //
-// What bounds it: 4 bytes of memory traffic an element. The angles of a token serve all of its heads, so a block takes a few
-// tokens whole: it starts the loads of its first elements, works out the cosines and sines of its tokens into shared memory
-// meanwhile, and then streams the heads through, 16 elements a thread. (A table of cosines and sines in memory would add 8
-// bytes a pair and a lookup; here a pair costs one sincos for 20 to 40 heads.)
+// What bounds it: 4 bytes of memory traffic an element. The angles of a token serve all of its heads: a warp starts the loads of
+// its first heads, works out the cosines and sines of its token meanwhile, one sincos a pair, and then streams the heads
+// through. (A table of cosines and sines in memory would add 8 bytes a pair and a lookup.)
 //
 // Angles: a position of 2^20 times a frequency of 1 in 32 bits is off by 0.03 to 0.06 rad. The frequency goes, by way of fp64,
 // into turns as a fixed-point fraction of 64 bits; times the position, modulo 2^64, that is the angle's fraction of a turn, off by
@@ -20,7 +19,7 @@ namespace fa2 {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 
 // cos and sin of position * frequency.
 __device__ __forceinline__ float2 turn_of(int64_t position, float frequency) {
@@ -109,95 +108,70 @@ __device__ __forceinline__ Head head_of(const RotaryParams& p, int b, int s, int
   return r;
 }
 
-// 16 bytes at a time: every row 16-byte aligned, pairs a multiple of 8. An item is 16 elements: 8 pairs, or 16 (at a head's end 8)
-// elements that are copied.
+// 16 bytes at a time: every row 16-byte aligned, pairs a multiple of 8. A lane has 16 elements of a head: 8 pairs, or 16 (at a head's
+// end 8) elements that are copied. A warp takes a token, or with few tokens 1 / 2^warps_log of a token's heads, and goes through the
+// heads with its pairs' cosines and sines in registers.
 template <bool BF16, bool NEIGHBOURS, bool APPEND>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryParams p) {
-  extern __shared__ __align__(16) float s_turn[];  // [token][cos 0-3, cos 4-7, sin 0-3, sin 4-7][chunk of 8 pairs][4]
-  __shared__ longlong2 s_row[32];
-  const int tid = threadIdx.x;
-  const int chunks = p.pairs / 8, n = p.pairs;
+__global__ void __launch_bounds__(kThreads, 8) rotary_kernel(const __grid_constant__ RotaryParams p) {
+  __shared__ __align__(16) float s_turn[kThreads / 32][2][128];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   early_wait();
   early_trigger();
-  const int first = blockIdx.x * p.tokens_per_block;
-  const int tokens = min(p.tokens_per_block, p.tokens - first);
-  const int total = tokens * static_cast<int>(p.heads_all.d * p.items.d);
+  const int w = blockIdx.x * (kThreads / 32) + warp, token = w >> p.warps_log;
+  if (token >= p.tokens) return;
+  const int b = p.seqlen.div(token), s = token - b * static_cast<int>(p.seqlen.d);
+  const int items = static_cast<int>(p.items.d), at_once = 32 / items;  // heads of a warp at a time
+  const int mine = lane / items, c = lane - mine * items, chunks = p.pairs / 8, n = p.pairs;
+  const bool pairs = c < chunks;
+  const int e0 = pairs && !NEIGHBOURS ? 8 * c : 16 * c, e1 = pairs && !NEIGHBOURS ? n + 8 * c : 16 * c + 8;
+  const int heads = static_cast<int>(p.heads_all.d), step = at_once << p.warps_log;
+  int h0 = mine < at_once ? (w & ((1 << p.warps_log) - 1)) * at_once + mine : heads;
 
-  struct Item {
-    int token, b, s, h, c;
-  };
-  auto item = [&](int i) {
-    Item r;
-    const int row = p.items.div(i);
-    r.c = i - row * static_cast<int>(p.items.d);
-    r.token = p.heads_all.div(row);
-    r.h = row - r.token * static_cast<int>(p.heads_all.d);
-    const int t = first + r.token;
-    r.b = p.seqlen.div(t);
-    r.s = t - r.b * static_cast<int>(p.seqlen.d);
-    return r;
-  };
-  auto places = [&](const Item& r, bool turned, int& e0, int& e1) {
-    if (turned && r.c < chunks) {
-      e0 = NEIGHBOURS ? 16 * r.c : 8 * r.c;
-      e1 = NEIGHBOURS ? e0 + 8 : n + e0;
-    } else {  // behind the turned elements 16 at a time; in a head that is only copied from the start
-      e0 = 16 * r.c;
-      e1 = e0 + 8;
-    }
-  };
-  constexpr int kBatch = 4;
-  uint4 w0[kBatch], w1[kBatch];
-  auto load = [&](int i0) {
+  // Heads that are loaded together; while they are turned, the loads of as many more are in flight. With 64 registers a thread, 32
+  // warps to an SM, one is best: forward of B4 S8192 H32/8 D128 109 us, of B2 S4093 H16/16 25.4; two 113 and 27.7 (80 registers);
+  // four at a time and none ahead 150 and 32.
+  constexpr int kBatch = 1;
+  uint4 w0[2][kBatch], w1[2][kBatch];
+  // A head that is only copied (a value) has its elements in their order.
+  auto first_of = [&](bool turned) { return turned ? e0 : 16 * c; };
+  auto second_of = [&](bool turned) { return turned ? e1 : 16 * c + 8; };
+  auto load = [&](int set, int h) {
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const int i = i0 + u * kThreads;
-      if (i < total) {
-        const Item r = item(i);
-        const Head h = head_of<APPEND>(p, r.b, r.s, r.h, make_longlong2(0, 0));
-        int e0, e1;
-        places(r, h.turned, e0, e1);
-        w0[u] = *reinterpret_cast<const uint4*>(h.in + e0);
-        if (e1 < p.head_dim) w1[u] = *reinterpret_cast<const uint4*>(h.in + e1);
+    for (int u = 0; u < kBatch; ++u)
+      if (h + u * step < heads) {
+        const Head x = head_of<APPEND>(p, b, s, h + u * step, make_longlong2(0, 0));
+        w0[set][u] = *reinterpret_cast<const uint4*>(x.in + first_of(x.turned));
+        if (second_of(x.turned) < p.head_dim) w1[set][u] = *reinterpret_cast<const uint4*>(x.in + second_of(x.turned));
       }
-    }
   };
-  load(tid);
-  for (int i = tid; i < tokens * n; i += kThreads) {
-    const int token = i / n, pair = i - token * n;
-    const int t = first + token, b = p.seqlen.div(t);
-    const float2 cs = turn_of_pair(p, b, t - b * static_cast<int>(p.seqlen.d), pair);
-    const int at = ((token * 4 + (pair & 7) / 4) * chunks + pair / 8) * 4 + (pair & 3);
-    s_turn[at] = cs.x;
-    s_turn[at + 2 * chunks * 4] = cs.y;
+  load(0, h0);
+  for (int i = lane; i < n; i += 32) {
+    const float2 cs = turn_of_pair(p, b, s, i);
+    s_turn[warp][0][i] = cs.x;
+    s_turn[warp][1][i] = cs.y;
   }
-  if (APPEND && tid < tokens) {
-    const int t = first + tid, b = p.seqlen.div(t);
-    s_row[tid] = cache_row(p, t, b, t - b * static_cast<int>(p.seqlen.d));
+  longlong2 row = make_longlong2(0, 0);
+  if constexpr (APPEND) row = cache_row(p, token, b, s);
+  __syncwarp();
+  float cs[16];  // cosines, then sines
+  if (pairs) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float4 f = *reinterpret_cast<const float4*>(&s_turn[warp][k >> 1][8 * c + 4 * (k & 1)]);
+      cs[4 * k] = f.x;
+      cs[4 * k + 1] = f.y;
+      cs[4 * k + 2] = f.z;
+      cs[4 * k + 3] = f.w;
+    }
   }
-  __syncthreads();
-  for (int i0 = tid; i0 < total; i0 += kBatch * kThreads) {
-    if (i0 != tid) load(i0);
+  auto turn = [&](int set, int first) {
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-      const int i = i0 + u * kThreads;
-      if (i >= total) break;
-      const Item r = item(i);
-      const Head h = head_of<APPEND>(p, r.b, r.s, r.h, APPEND ? s_row[r.token] : make_longlong2(0, 0));
-      if (APPEND && h.out == nullptr) continue;
-      int e0, e1;
-      places(r, h.turned, e0, e1);
-      uint32_t a[8] = {w0[u].x, w0[u].y, w0[u].z, w0[u].w, w1[u].x, w1[u].y, w1[u].z, w1[u].w};
-      if (h.turned && r.c < chunks) {
-        float cs[16];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float4 f = *reinterpret_cast<const float4*>(s_turn + ((r.token * 4 + k) * chunks + r.c) * 4);
-          cs[4 * k] = f.x;
-          cs[4 * k + 1] = f.y;
-          cs[4 * k + 2] = f.z;
-          cs[4 * k + 3] = f.w;
-        }
+      if (first + u * step >= heads) break;
+      const Head h = head_of<APPEND>(p, b, s, first + u * step, row);
+      const uint4 x0 = w0[set][u], x1 = w1[set][u];
+      uint32_t a[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+      if (h.turned && pairs) {
         if constexpr (NEIGHBOURS) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
@@ -214,9 +188,16 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
           }
         }
       }
-      *reinterpret_cast<uint4*>(h.out + e0) = make_uint4(a[0], a[1], a[2], a[3]);
-      if (e1 < p.head_dim) *reinterpret_cast<uint4*>(h.out + e1) = make_uint4(a[4], a[5], a[6], a[7]);
+      if (APPEND && h.out == nullptr) continue;
+      *reinterpret_cast<uint4*>(h.out + first_of(h.turned)) = make_uint4(a[0], a[1], a[2], a[3]);
+      if (second_of(h.turned) < p.head_dim) *reinterpret_cast<uint4*>(h.out + second_of(h.turned)) = make_uint4(a[4], a[5], a[6], a[7]);
     }
+  };
+  for (; h0 < heads; h0 += 2 * kBatch * step) {
+    load(1, h0 + kBatch * step);
+    turn(0, h0);
+    load(0, h0 + 2 * kBatch * step);
+    turn(1, h0 + kBatch * step);
   }
 }
 
@@ -256,16 +237,16 @@ __global__ void __launch_bounds__(kThreads) rotary_any_kernel(const __grid_const
 template <bool BF16, bool APPEND>
 cudaError_t pick(const RotaryParams& p, bool vectors, cudaStream_t stream) {
   if (!vectors) return launch_grid(true, rotary_any_kernel<BF16, APPEND>, dim3(p.tokens), kThreads, 0, stream, p);
-  const int grid = (p.tokens + p.tokens_per_block - 1) / p.tokens_per_block;
-  const size_t smem = static_cast<size_t>(p.tokens_per_block) * p.pairs * 8;
-  if (p.neighbours) return launch_grid(true, rotary_kernel<BF16, true, APPEND>, dim3(grid), kThreads, smem, stream, p);
-  return launch_grid(true, rotary_kernel<BF16, false, APPEND>, dim3(grid), kThreads, smem, stream, p);
+  const int64_t warps = static_cast<int64_t>(p.tokens) << p.warps_log;
+  const dim3 grid(static_cast<unsigned>((warps + kThreads / 32 - 1) / (kThreads / 32)));
+  if (p.neighbours) return launch_grid(true, rotary_kernel<BF16, true, APPEND>, grid, kThreads, 0, stream, p);
+  return launch_grid(true, rotary_kernel<BF16, false, APPEND>, grid, kThreads, 0, stream, p);
 }
 
 }  // namespace
 
 cudaError_t launch_rotary(const RotaryParams& p, bool bf16, bool append, bool vectors, cudaStream_t stream) {
-  if (p.tokens <= 0 || p.tokens_per_block <= 0 || p.tokens_per_block > 32 || p.pairs < 0 || p.pairs > 128) return cudaErrorInvalidValue;
+  if (p.tokens <= 0 || p.warps_log < 0 || p.warps_log > 8 || p.pairs < 0 || p.pairs > 128) return cudaErrorInvalidValue;
   if (append) return bf16 ? pick<true, true>(p, vectors, stream) : pick<false, true>(p, vectors, stream);
   return bf16 ? pick<true, false>(p, vectors, stream) : pick<false, false>(p, vectors, stream);
 }
