@@ -191,13 +191,9 @@ class RotaryAxes : public torch::autograd::Function<RotaryAxes> {
     }
     if (ctx != nullptr) {
       ctx->save_for_backward({positions, inv_freq});
-      auto& d = ctx->saved_data;
-      d["sections"] = std::vector<int64_t>(turn.sections.begin(), turn.sections.begin() + turn.axes);
-      d["interleaved_axes"] = turn.interleaved_axes;
-      d["interleaved_pairs"] = turn.interleaved_pairs;
-      d["inverse"] = inverse;
-      d["q"] = q.defined();
-      d["k"] = k.defined();
+      std::vector<int64_t> d(turn.sections.begin(), turn.sections.begin() + turn.axes);
+      d.insert(d.end(), {turn.interleaved_axes, turn.interleaved_pairs, inverse, q.defined(), k.defined()});
+      ctx->saved_data["turn"] = std::move(d);
     }
     torch::autograd::variable_list out;
     if (q_out.defined()) out.push_back(q_out);
@@ -206,21 +202,22 @@ class RotaryAxes : public torch::autograd::Function<RotaryAxes> {
   }
   // The turn back, which is this function again: it has gradients of its own.
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
-    auto& d = ctx->saved_data;
     const auto saved = ctx->get_saved_variables();
+    const auto d = ctx->saved_data["turn"].toIntVector();
     Turn turn;
-    const auto sections = d["sections"].toIntVector();
-    turn.axes = static_cast<int>(sections.size());
-    for (int i = 0; i < turn.axes; ++i) turn.pairs += turn.sections[i] = static_cast<int32_t>(sections[i]);
-    turn.interleaved_axes = d["interleaved_axes"].toBool();
-    turn.interleaved_pairs = d["interleaved_pairs"].toBool();
-    const bool has_q = d["q"].toBool(), has_k = d["k"].toBool();
+    turn.axes = static_cast<int>(d.size()) - 5;
+    for (int i = 0; i < turn.axes; ++i) turn.pairs += turn.sections[i] = static_cast<int32_t>(d[i]);
+    const int64_t* rest = d.data() + turn.axes;
+    turn.interleaved_axes = rest[0];
+    turn.interleaved_pairs = rest[1];
+    const bool inverse = rest[2], has_q = rest[3], has_k = rest[4];
     Tensor dq, dk;
     if (has_q && ctx->needs_input_grad(0)) dq = grads[0];
     if (has_k && ctx->needs_input_grad(has_q)) dk = grads[has_q];
     torch::autograd::variable_list result(6);
     if (!dq.defined() && !dk.defined()) return result;
-    auto turned = apply(some(dq), some(dk), saved[0], saved[1], turn, !d["inverse"].toBool());
+    auto turned = at::GradMode::is_enabled() ? apply(some(dq), some(dk), saved[0], saved[1], turn, !inverse)
+                                             : forward(nullptr, some(dq), some(dk), saved[0], saved[1], turn, !inverse);
     if (dq.defined()) result[0] = turned.front();
     if (dk.defined()) result[1] = turned.back();
     return result;
