@@ -143,8 +143,8 @@ int rotary_launch(fa2::RotaryParams* p, int dtype, bool append, bool vectors, Ru
 struct FwdPlan {
   int most_keys = 0, rows = 0, row_tiles = 0, grid = 0;
   int64_t score_stride = 0;
-  int64_t list_bytes = 0, part_bytes = 0, stat_bytes = 0, score_bytes = 0;
-  int64_t bytes() const { return list_bytes + part_bytes + stat_bytes + score_bytes; }
+  int64_t list_bytes = 0, part_bytes = 0, unit_bytes = 0, stat_bytes = 0, score_bytes = 0;
+  int64_t bytes() const { return list_bytes + part_bytes + unit_bytes + stat_bytes + score_bytes; }
 };
 int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
 
@@ -162,6 +162,7 @@ int plan_fwd(const fa2_paged_fwd_args* a, int sm_count, FwdPlan* f) {
   if (c->attn_mass != nullptr) {
     const int64_t rows = static_cast<int64_t>(c->batch) * c->heads_k * f->rows;
     f->score_stride = (f->most_keys + 15) / 16 * 16;
+    f->unit_bytes = round256(static_cast<int64_t>(c->batch) * c->heads_k * f->row_tiles * 8);
     f->stat_bytes = round256(rows * 8);
     if (rows > (INT64_MAX >> 8) / f->score_stride) return fail(FA2_E_VALUE, "the scores of this call do not fit an address space");
     f->score_bytes = round256(rows * f->score_stride * 4);
@@ -304,14 +305,14 @@ int fa2_paged_fwd(const fa2_paged_fwd_args* args, void* workspace, int64_t works
   p.shared = reinterpret_cast<int4*>(at);
   p.partials = reinterpret_cast<float*>(at += f.list_bytes);
   if (c->attn_mass != nullptr) {
-    p.stats = reinterpret_cast<float2*>(at += f.part_bytes);
+    p.units = reinterpret_cast<int2*>(at += f.part_bytes);
+    p.stats = reinterpret_cast<float2*>(at += f.unit_bytes);
     p.scores = reinterpret_cast<float*>(at += f.stat_bytes);
     p.score_stride = f.score_stride;
     p.mass = c->attn_mass;
   }
   p.status = rt->status;
-  cudaError_t e = fa2::launch_fwd_paged(p, f.grid, c->dtype == FA2_BF16, static_cast<cudaStream_t>(stream));
-  if (e == cudaSuccess && p.mass != nullptr) e = fa2::launch_paged_mass(p, rt->sm_count, static_cast<cudaStream_t>(stream));
+  const cudaError_t e = fa2::launch_fwd_paged(p, f.grid, rt->sm_count, c->dtype == FA2_BF16, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return fail(FA2_E_RUNTIME, "paged forward launch failed: %s", cudaGetErrorString(e));
   return FA2_OK;
 }

@@ -63,7 +63,8 @@ struct PagedParams {
   int4* shared;                 // of the unit that begins in a CTA's share and ends in another: its parts (0: there is none), sequence, kv head, row tile
   float* scores;                // [batch, heads_k, rows, score_stride] in the log2 domain, or null
   int64_t score_stride;
-  float2* stats;                // [batch, heads_k, rows]: row maximum (log2 domain), 1 / row sum
+  float2* stats;                // [batch, heads_k, rows]: row maximum (log2 domain), 1 / row sum, where one CTA has the row's unit
+  int2* units;                  // [batch, heads_k, row_tiles]: first CTA and number of its parts (0: it is whole)
   float* mass;                  // [pages, heads_k, page_size]
   int* status;
 };
@@ -92,8 +93,7 @@ inline int paged_unit_rows(int head_dim, int rows) { return rows <= 8 ? 8 : rows
 inline int64_t paged_part_floats(int head_dim, int rows) {
   return paged_unit_rows(head_dim, rows) * (static_cast<int64_t>((head_dim + 63) / 64 * 64) + 2);
 }
-cudaError_t launch_fwd_paged(const PagedParams& p, int grid, bool bf16, cudaStream_t stream);
-cudaError_t launch_paged_mass(const PagedParams& p, int sm_count, cudaStream_t stream);
+cudaError_t launch_fwd_paged(const PagedParams& p, int grid, int sm_count, bool bf16, cudaStream_t stream);
 
 cudaError_t launch_paged_evict(const EvictParams& p, int sm_count, cudaStream_t stream);
 

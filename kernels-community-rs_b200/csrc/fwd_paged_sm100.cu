@@ -8,7 +8,7 @@
 //   * The query rows of a kv head (row r = query r / group, head r % group) are the M of one product, 16 at a time.
 //   * The lengths are on the device. Every CTA, one per SM, adds up the sequences' key tiles and takes an equal share of the list
 //     of all (sequence, kv head, key tile); a share may begin and end inside a unit. A CTA leaves its part of a unit that it does
-//     not cover alone in the workspace, and a second kernel, which waits beside the first, adds the parts up.
+//     not cover alone in the workspace, and a second kernel, which waits beside the first, adds the parts up (and the keys' weights).
 //   * A thread's copies are its own. mma.sync takes B fragments whose k index may be permuted freely as long as A's is alike, and
 //     n is only a name; so lane (g, t) = (lane / 4, lane % 4) takes 16-byte pieces t, t + 4, ... of key g's row as two k-steps of
 //     Q K^T, and pieces g, g + 8, ... of the rows of keys 2t, 2t + 1, 2t + 8, 2t + 9 as columns of P V. Every lane therefore reads
@@ -634,7 +634,10 @@ __global__ void __launch_bounds__((Cfg<A, NT>::kThreads), 1) fwd_paged_kernel(co
       }
       __syncthreads();
     }
-    // The unit that begins in this share and ends in another is paged_join_kernel's, and known there by this CTA.
+    // A unit that this CTA begins is known by it to paged_tail_kernel: in how many parts it comes.
+    if (p.units != nullptr && done.j0 == 0 && tid == 0)
+      p.units[(static_cast<int64_t>(done.b) * p.heads_k + done.hk) * p.row_tiles + done.rt] =
+          make_int2(blockIdx.x, whole ? 0 : share_owner(done.start + done.tiles - 1, n_tiles, ctas) - static_cast<int>(blockIdx.x) + 1);
     if (!more && tid == 0) {
       const int c_last = share_owner(done.start + done.tiles - 1, n_tiles, ctas);
       p.shared[blockIdx.x] = make_int4(whole || done.j0 > 0 ? 0 : c_last - static_cast<int>(blockIdx.x) + 1, done.b, done.hk, done.rt);
@@ -650,23 +653,26 @@ __global__ void __launch_bounds__((Cfg<A, NT>::kThreads), 1) fwd_paged_kernel(co
   if (tid == 0) report_abort(&s_abort, p.status);
 }
 
-// The units that several CTAs share: block (c, y) adds up the parts of 8 rows of the one that begins in share c, in the order of the
-// keys. A kernel of its own, which starts early and waits beside the attention. (With flags in memory, by which the last CTA of a unit
-// knew itself, a call ended with two fences and two round trips to memory: B1 H32/8 Sk 8192 D128 17.3 us in place of 14.9.)
-constexpr int kJoinThreads = 128;  // its registers fit beside those of the attention
+// ---- what is left when the parts are there: the units that several CTAs share, and the weights. A kernel of its own, which starts
+// early and waits beside the attention. (With flags in memory, by which the last CTA of a unit knew itself, a call ended with two fences
+// and two round trips to memory: B1 H32/8 Sk 8192 D128 17.3 us in place of 14.9.)
+constexpr int kTailThreads = 128;  // its registers fit beside those of the attention
+
+// Slot 2 c holds the part of a segment that began before CTA c's share, 2 c + 1 that of one that began in it: the first part.
+__device__ __forceinline__ const float* part_of(const PagedParams& p, int c_first, int i, int64_t slot) {
+  return p.partials + (2 * static_cast<int64_t>(c_first + i) + (i == 0 ? 1 : 0)) * slot;
+}
+
+// Adds up the parts of 8 rows (from `first_row` on) of the unit that begins in share c, in the order of the keys.
 template <bool BF16>
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedParams p, int d, int unit_rows) {
-  early_wait();
-  early_trigger();
-  const int4 unit = p.shared[blockIdx.x];
+__device__ __forceinline__ void join_parts(const PagedParams& p, int c, int first_row, int d, int unit_rows) {
+  const int4 unit = p.shared[c];
   const int n_parts = unit.x;
   if (n_parts == 0) return;
-  const int row0 = unit.w * unit_rows + blockIdx.y * 8, rows = min(8, min(unit_rows - static_cast<int>(blockIdx.y) * 8, p.rows - row0));
+  const int row0 = unit.w * unit_rows + first_row, rows = min(8, min(unit_rows - first_row, p.rows - row0));
   const int64_t slot = static_cast<int64_t>(unit_rows) * (d + 2);
-  // Slot 2 c holds a segment that began before CTA c's share, 2 c + 1 one that began in it: the first part.
-  const float* first = p.partials + (2 * static_cast<int64_t>(blockIdx.x) + 1) * slot;
-  for (int i = threadIdx.x; i < rows * (d / 4); i += kJoinThreads) {
-    const int r = blockIdx.y * 8 + i / (d / 4), col = i % (d / 4) * 4;
+  for (int i = threadIdx.x; i < rows * (d / 4); i += kTailThreads) {
+    const int r = first_row + i / (d / 4), col = i % (d / 4) * 4;
     float top = -INFINITY, total = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     constexpr int kBatch = 10;  // parts whose loads are in flight together
@@ -677,7 +683,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
       for (int e = 0; e < kBatch; ++e) {
         pm[e] = -INFINITY;
         if (c0 + e < n_parts) {
-          const float* src = first + (c0 + e == 0 ? 0 : 2 * (c0 + e) - 1) * slot;
+          const float* src = part_of(p, c, c0 + e, slot);
           v[e] = __ldcg(reinterpret_cast<const float4*>(src + r * d + col));
           pm[e] = __ldcg(src + unit_rows * d + r);
           pl[e] = __ldcg(src + unit_rows * d + unit_rows + r);
@@ -705,31 +711,72 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
   }
 }
 
-// mass[page][kv head][row] += sum over the query rows of exp2(score - maximum) / sum. One thread a key; the sum is in the order of
-// the rows, and the addition is atomic because sequences may share a page.
-template <int kMassThreads>
-__global__ void __launch_bounds__(kMassThreads) paged_mass_kernel(const __grid_constant__ PagedParams p) {
+// mass[page][kv head][row] += sum over the query rows of exp2(score - maximum) / sum, four keys a thread; the sum is in the order of
+// the rows, and the addition is atomic because sequences may share a page. The rows' maxima and sums are those of the unit where
+// one CTA has it, else they come from the parts.
+__device__ __forceinline__ void add_weights(const PagedParams& p, int unit, int block, int blocks, int d, int unit_rows, float2* s_stats) {
+  const int b = unit / p.heads_k, hk = unit - b * p.heads_k;
+  const int length = cut_length(p.seqlens[b], min(static_cast<int64_t>(p.most_keys), p.table.capacity()));
+  const int lo = p.window < 0 ? 0 : max(0, length - p.seqlen_q - p.window);
+  const int64_t step = 4 * static_cast<int64_t>(blocks) * kTailThreads;
+  int64_t key = lo / 4 * 4 + 4 * (static_cast<int64_t>(block) * kTailThreads + threadIdx.x);
+  if (key - 4 * threadIdx.x >= length) return;
+  const int64_t slot = static_cast<int64_t>(unit_rows) * (d + 2);
+  for (int r = threadIdx.x; r < p.rows; r += kTailThreads) {
+    const int rt = r / unit_rows, in = r - rt * unit_rows;
+    const int2 parts = p.units[static_cast<int64_t>(unit) * p.row_tiles + rt];
+    float2 stat;
+    if (parts.y == 0) {
+      stat = __ldcg(p.stats + static_cast<int64_t>(unit) * p.rows + r);
+    } else {
+      float top = -INFINITY, total = 0.f;
+#pragma unroll 8
+      for (int i = 0; i < parts.y; ++i) {
+        const float* src = part_of(p, parts.x, i, slot) + unit_rows * d + in;
+        const float m = __ldcg(src), l = __ldcg(src + unit_rows), above = fmaxf(top, m);
+        total = total * part_scale(top, above) + l * part_scale(m, above);
+        top = above;
+      }
+      stat = make_float2(top, total == 0.f ? 0.f : 1.f / total);
+    }
+    s_stats[r] = stat;
+  }
+  __syncthreads();
+  const bool by_four = p.table.page_size.d % 4 == 0;
+  for (; key < length; key += step) {
+    const float* from = p.scores + static_cast<int64_t>(unit) * p.rows * p.score_stride + key;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int r = 0; r < p.rows; ++r) {
+      const float4 s = __ldcg(reinterpret_cast<const float4*>(from + r * p.score_stride));
+      const float2 stat = s_stats[r];
+      auto weight = [&](float x) { return x == -INFINITY ? 0.f : ex2(x - stat.x) * stat.y; };
+      sum[0] += weight(s.x), sum[1] += weight(s.y), sum[2] += weight(s.z), sum[3] += weight(s.w);
+    }
+    int page = -1;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int at = static_cast<int>(key) + e;
+      if (at < lo || at >= length) continue;
+      if (page < 0 || !by_four) page = p.table.page_of(b, at);
+      if (page >= 0)
+        atomicAdd(p.mass + (static_cast<int64_t>(page) * p.heads_k + hk) * p.table.page_size.d + p.table.page_size.mod(at), sum[e]);
+    }
+  }
+}
+
+// Blocks: `joins` for the shared units, 8 rows each, then `blocks` for the weights of each (sequence, kv head).
+template <bool BF16>
+__global__ void __launch_bounds__(kTailThreads) paged_tail_kernel(const __grid_constant__ PagedParams p, int grid, int joins, int blocks, int d, int unit_rows) {
   __shared__ float2 s_stats[kPagedMaxRows];
   early_wait();
   early_trigger();
-  const int unit = blockIdx.x, b = unit / p.heads_k, hk = unit - b * p.heads_k;
-  const int length = cut_length(p.seqlens[b], min(static_cast<int64_t>(p.most_keys), p.table.capacity()));
-  const int64_t lo = p.window < 0 ? 0 : max(static_cast<int64_t>(length) - p.seqlen_q - p.window, static_cast<int64_t>(0));
-  const int64_t step = static_cast<int64_t>(gridDim.y) * kMassThreads;
-  if (lo / 16 * 16 + blockIdx.y * kMassThreads >= length) return;
-  for (int r = threadIdx.x; r < p.rows; r += kMassThreads) s_stats[r] = __ldcg(p.stats + static_cast<int64_t>(unit) * p.rows + r);
-  __syncthreads();
-  for (int64_t key = lo / 16 * 16 + blockIdx.y * kMassThreads + threadIdx.x; key < length; key += step) {
-    if (key < lo) continue;
-    const float* from = p.scores + static_cast<int64_t>(unit) * p.rows * p.score_stride + key;
-    float sum = 0.f;
-    for (int r = 0; r < p.rows; ++r) {
-      const float s = __ldcg(from + r * p.score_stride);
-      if (s != -INFINITY) sum += ex2(s - s_stats[r].x) * s_stats[r].y;
-    }
-    const int page = p.table.page_of(b, static_cast<int>(key));
-    if (page >= 0)
-      atomicAdd(p.mass + (static_cast<int64_t>(page) * p.heads_k + hk) * p.table.page_size.d + p.table.page_size.mod(static_cast<int>(key)), sum);
+  const int i = blockIdx.x;
+  if (i < joins) {
+    join_parts<BF16>(p, i % grid, i / grid * 8, d, unit_rows);
+  } else {
+    const int unit = (i - joins) / blocks;
+    add_weights(p, unit, i - joins - unit * blocks, blocks, d, unit_rows, s_stats);
   }
 }
 
@@ -772,24 +819,18 @@ cudaError_t pick_dim(const PagedParams& p, int grid, cudaStream_t stream) {
 
 }  // namespace
 
-cudaError_t launch_fwd_paged(const PagedParams& p, int grid, bool bf16, cudaStream_t stream) {
+cudaError_t launch_fwd_paged(const PagedParams& p, int grid, int sm_count, bool bf16, cudaStream_t stream) {
   if (p.rows <= 0 || p.rows > kPagedMaxRows || p.head_dim <= 0 || p.head_dim > 256 || grid <= 0) return cudaErrorInvalidValue;
   const cudaError_t e = bf16 ? pick_dim<true>(p, grid, stream) : pick_dim<false>(p, grid, stream);
   if (e != cudaSuccess) return e;
-  const int d = (p.head_dim + 63) / 64 * 64, unit_rows = paged_unit_rows(p.head_dim, p.rows);
-  const dim3 blocks(grid, (unit_rows + 7) / 8);
-  if (bf16) return launch_grid(true, paged_join_kernel<true>, blocks, kJoinThreads, 0, stream, p, d, unit_rows);
-  return launch_grid(true, paged_join_kernel<false>, blocks, kJoinThreads, 0, stream, p, d, unit_rows);
-}
-
-cudaError_t launch_paged_mass(const PagedParams& p, int sm_count, cudaStream_t stream) {
-  constexpr int kMassThreads = 256;
-  const int units = p.batch * p.heads_k;
-  const int64_t blocks = (static_cast<int64_t>(p.most_keys) + 15 + kMassThreads - 1) / kMassThreads;
+  const int d = (p.head_dim + 63) / 64 * 64, unit_rows = paged_unit_rows(p.head_dim, p.rows), joins = grid * (unit_rows / 8);
   // Blocks for every key that there can be, but no more than fill the GPU a few times over: lengths are known on the device only.
-  const int64_t most = (16 * static_cast<int64_t>(sm_count) + units - 1) / units;
-  const int y = static_cast<int>(blocks < most ? blocks : most);
-  return launch_grid(true, paged_mass_kernel<kMassThreads>, dim3(units, y), kMassThreads, 0, stream, p);
+  const int64_t units = static_cast<int64_t>(p.batch) * p.heads_k, keys = 4 * kTailThreads;
+  const int64_t every = (static_cast<int64_t>(p.most_keys) + 3 + keys - 1) / keys, fill = (32 * static_cast<int64_t>(sm_count) + units - 1) / units;
+  const int blocks = p.mass != nullptr ? static_cast<int>(every < fill ? every : fill) : 0;
+  const dim3 all(static_cast<unsigned>(joins + units * blocks));
+  if (bf16) return launch_grid(true, paged_tail_kernel<true>, all, kTailThreads, 0, stream, p, grid, joins, blocks, d, unit_rows);
+  return launch_grid(true, paged_tail_kernel<false>, all, kTailThreads, 0, stream, p, grid, joins, blocks, d, unit_rows);
 }
 
 }  // namespace fa2

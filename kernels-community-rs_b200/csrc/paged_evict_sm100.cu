@@ -7,12 +7,17 @@
 // What bounds it: reading the weights once, and reading and writing the rows that are kept (8 D bytes a row of keys and values).
 // Two kernels:
 //
-//   * The choice, a CTA per (sequence, kv head): the weights become 32-bit keys in the order of the numbers, in shared memory
-//     while they fit. A radix search from the top (11, 11 and 10 bits, a histogram each) finds the key of the last one to be
-//     kept and how many of the keys equal to it are; one pass in the order of the tokens then writes the list of what is kept.
-//   * The move, all SMs: a row's 16-byte pieces by neighbouring threads, eight pieces in flight per thread. Sources and
-//     destinations are different pages, so that the rows can move in any order and pages shared with another sequence stay as
-//     they are.
+//   * The choice, a cluster of 1 to 8 CTAs per (sequence, kv head), so that few of them use more of the GPU. The weights become
+//     32-bit keys in the order of the numbers, 16 of them in each thread's registers; what does not fit is read again in every
+//     pass. A radix search from the top (11, 11 and 10 bits, a histogram each, the CTAs' added up over distributed shared memory)
+//     finds the key of the last one to be kept and how many of the keys equal to it are; one pass in the order of the tokens
+//     then writes the list of what is kept. It is bound by the latency of its steps: B2 Hk8 from 4096 tokens 12 us with one CTA each.
+//   * The move, all SMs: a row's 16-byte pieces by neighbouring threads, one of K and one of V in flight in each of 2048 threads per
+//     SM. (Two or four rows a thread, and fewer threads, are slower: B16 Hk4 16384 -> 6000 87 and 92 us a call in place of 83.)
+//     Sources and destinations are different pages, so that the rows can move in any order and pages shared with another
+//     sequence stay as they are.
+#include <algorithm>
+
 #include "sm100_ptx.cuh"
 #include "fa2_launch.h"
 #include "fa2_paged_params.h"
@@ -22,9 +27,9 @@ namespace fa2 {
 namespace {
 
 constexpr int kSelectThreads = 1024;
-constexpr int kSelectWarps = kSelectThreads / 32;
 constexpr int kBins = 2048;
-constexpr int kHeld = 48 * 1024;   // keys that shared memory holds
+constexpr int kRounds = 4;                            // groups of four neighbouring keys that a thread holds
+constexpr int kRoundKeys = 4 * kSelectThreads;
 
 // Larger numbers have larger keys; both zeroes are one, and NaN is above all.
 __device__ __forceinline__ uint32_t order_key(float f) {
@@ -34,137 +39,274 @@ __device__ __forceinline__ uint32_t order_key(float f) {
   return u >> 31 ? ~u : u | 0x80000000u;
 }
 
-// Sum over the threads before this one, and over all.
-__device__ __forceinline__ int block_scan(int x, int* s_warp, int& all) {
+// x[i] becomes the sum over the threads before this one, all[i] the sum over all.
+// The last N - n of them are left out: they are zero.
+template <int N>
+__device__ __forceinline__ void block_scan(int (&x)[N], int (&all)[N], int n, int (*s_warp)[32]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int y = x;
+  int y[N];
 #pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int z = __shfl_up_sync(0xffffffffu, y, d);
-    if (lane >= d) y += z;
+  for (int i = 0; i < N; ++i) {
+    if (i >= n) break;
+    y[i] = x[i];
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int z = __shfl_up_sync(0xffffffffu, y[i], d);
+      if (lane >= d) y[i] += z;
+    }
   }
   __syncthreads();
-  if (lane == 31) s_warp[warp] = y;
-  __syncthreads();
-  int w = s_warp[lane];
+  if (lane == 31) {
 #pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int z = __shfl_up_sync(0xffffffffu, w, d);
-    if (lane >= d) w += z;
+    for (int i = 0; i < N; ++i)
+      if (i < n) s_warp[i][warp] = y[i];
   }
-  all = __shfl_sync(0xffffffffu, w, 31);
-  const int before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
-  return y - x + (warp > 0 ? before : 0);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    all[i] = 0;
+    if (i >= n) continue;
+    int w = s_warp[i][lane];
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int z = __shfl_up_sync(0xffffffffu, w, d);
+      if (lane >= d) w += z;
+    }
+    all[i] = __shfl_sync(0xffffffffu, w, 31);
+    const int before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
+    x[i] = y[i] - x[i] + (warp > 0 ? before : 0);
+  }
 }
-static_assert(kSelectWarps == 32, "the scan takes one warp sum a lane");
+static_assert(kSelectThreads == 32 * 32, "the scan takes one warp sum a lane");
 
-// HELD: the table has room for no more tokens than shared memory has for keys. Otherwise a sequence whose keys fit after all still has
-// them there, and those of a longer one are read again in every pass.
-template <bool HELD>
+// Four neighbouring words of the shared memory of the cluster's CTA `rank`.
+__device__ __forceinline__ int4 peer_words(const int* word, uint32_t rank) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(peer_smem(smem_u32(word), rank)) : "memory");
+  return v;
+}
+
+template <int CTAS>
 __global__ void __launch_bounds__(kSelectThreads, 1) evict_select_kernel(const __grid_constant__ EvictParams p) {
-  extern __shared__ uint32_t s_key[];
-  __shared__ int s_bin[kBins];
-  __shared__ int s_warp[32];
+  __shared__ __align__(16) int s_bin[3][kBins];   // one for each pass: the other CTAs may still read the one before
+  __shared__ int s_warp[kRounds][32];
+  __shared__ __align__(16) int s_count[4];       // keys above and equal to the last one's
   __shared__ int s_found, s_above;
   const int tid = threadIdx.x;
-  const int b = blockIdx.x / p.heads_k, hk = blockIdx.x - b * p.heads_k;
+  const int unit = blockIdx.x / CTAS, rank = blockIdx.x - unit * CTAS;
+  const int b = unit / p.heads_k, hk = unit - b * p.heads_k;
+  for (int i = tid; i < 3 * kBins; i += kSelectThreads) s_bin[0][i] = 0;
   early_wait();
   early_trigger();
-  const int64_t most = min(p.from.capacity(), static_cast<int64_t>(INT32_MAX - 8 * kSelectThreads));
+  auto meet = [&]() {  // all threads of the cluster; what they wrote to shared memory is seen by all
+    __syncwarp();
+    if constexpr (CTAS > 1) {
+      cluster_arrive();
+      cluster_wait();
+    } else {
+      __syncthreads();
+    }
+  };
+  const int64_t most = min(p.from.capacity(), static_cast<int64_t>(INT32_MAX - 8 * kRoundKeys));
   const int given = p.seqlens[b];
   const int n = cut_length(given, most);
   if (tid == 0 && given > most && p.status != nullptr) atomicCAS(p.status, 0, static_cast<int>(kPagedTooLong));
-  int32_t* kept = p.kept + static_cast<int64_t>(blockIdx.x) * p.budget;
-  const int n_kept = min(n, p.budget);
-  if (hk == 0 && tid == 0) p.seqlens_out[b] = n_kept;
-  for (int i = n_kept + tid; i < p.budget; i += kSelectThreads) kept[i] = -1;
+  int32_t* kept = p.kept + static_cast<int64_t>(unit) * p.budget;
+  const int n_kept = min(n, p.budget), at = rank * kSelectThreads + tid;
+  if (hk == 0 && at == 0) p.seqlens_out[b] = n_kept;
+  for (int i = n_kept + at; i < p.budget; i += CTAS * kSelectThreads) kept[i] = -1;
   if (n <= p.budget) {
-    for (int i = tid; i < n; i += kSelectThreads) kept[i] = i;
+    for (int i = at; i < n; i += CTAS * kSelectThreads) kept[i] = i;
     return;
   }
   const int others = n - p.recent, wanted = p.budget - p.recent;  // wanted < others
-  for (int i = tid; i < p.recent; i += kSelectThreads) kept[wanted + i] = others + i;
+  for (int i = at; i < p.recent; i += CTAS * kSelectThreads) kept[wanted + i] = others + i;
   if (wanted == 0) return;
 
-  auto read = [&](int i) {
-    const int page = p.from.page_of(b, i);
-    if (page < 0) {
-      if (p.status != nullptr) atomicCAS(p.status, 0, static_cast<int>(kPagedBadPage));
-      return 0u;  // the first to go
-    }
-    return order_key(p.mass[(static_cast<int64_t>(page) * p.heads_k + hk) * p.from.page_size.d + p.from.page_size.mod(i)]);
+  // ---- this CTA's tokens, and their keys
+  const int slice = ((others + CTAS - 1) / CTAS + 3) / 4 * 4;
+  const int begin = min(others, rank * slice), end = min(others, begin + slice);
+  const bool by_four = p.from.page_size.d % 4 == 0 && reinterpret_cast<uintptr_t>(p.mass) % 16 == 0;  // four neighbours are on one page
+  auto weights = [&](int page) { return p.mass + (static_cast<int64_t>(page) * p.heads_k + hk) * p.from.page_size.d; };
+  auto no_page = [&]() {
+    if (p.status != nullptr) atomicCAS(p.status, 0, static_cast<int>(kPagedBadPage));
   };
-  const bool held = HELD || others <= kHeld;
-  if (held)
-    for (int i = tid; i < others; i += kSelectThreads) s_key[i] = read(i);
-  auto key_at = [&](int i) { return held ? s_key[i] : read(i); };
+  // Four tokens from i on; a token of a page that cannot be is the first to go.
+  auto read = [&](int i, uint32_t (&k)[4]) {
+    k[0] = k[1] = k[2] = k[3] = 0;
+    if (by_four) {
+      const int page = p.from.page_of(b, i);
+      if (page < 0) return no_page();
+      const float4 w = *reinterpret_cast<const float4*>(weights(page) + p.from.page_size.mod(i));
+      k[0] = order_key(w.x), k[1] = order_key(w.y), k[2] = order_key(w.z), k[3] = order_key(w.w);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (i + e < end) {
+          const int page = p.from.page_of(b, i + e);
+          if (page < 0) no_page();
+          else k[e] = order_key(weights(page)[p.from.page_size.mod(i + e)]);
+        }
+    }
+  };
+  const bool held = slice <= kRounds * kRoundKeys;
+  uint32_t key[kRounds][4];
+  if (held) {
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+      const int i = begin + r * kRoundKeys + 4 * tid;
+      if (i < end) read(i, key[r]);
+    }
+  }
+  // Calls f(first token, its four keys) for this thread's groups of four.
+  auto visit = [&](auto&& f) {
+    if (held) {
+#pragma unroll
+      for (int r = 0; r < kRounds; ++r) {
+        const int i = begin + r * kRoundKeys + 4 * tid;
+        if (i < end) f(i, key[r]);
+      }
+    } else {
+      for (int i = begin + 4 * tid; i < end; i += kRoundKeys) {
+        uint32_t k[4];
+        read(i, k);
+        f(i, k);
+      }
+    }
+  };
 
-  // ---- the key of the last one to be kept: `prefix` are its bits above `shift`, `above` counts the larger keys
+  // ---- the key of the last one to be kept: `prefix` are its bits so far, `above` counts the larger keys
   uint32_t prefix = 0;
   int above = 0;
+  __syncthreads();  // the histograms are clear
 #pragma unroll 1
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
-    for (int i = tid; i < kBins; i += kSelectThreads) s_bin[i] = 0;
-    __syncthreads();
-    for (int i = tid; i < others; i += kSelectThreads) {
-      const uint32_t k = key_at(i);
-      if (pass == 0 || k >> (shift + bits) == prefix) atomicAdd(&s_bin[(k >> shift) & ((1u << bits) - 1)], 1);
+    int* bin = s_bin[pass];
+    visit([&](int i, const uint32_t (&k)[4]) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (i + e < end && (pass == 0 || k[e] >> (shift + bits) == prefix)) atomicAdd(&bin[(k[e] >> shift) & ((1u << bits) - 1)], 1);
+    });
+    meet();
+    // Threads 0 to 255 have eight bins each, from the top.
+    int sum[8] = {}, mine = 0;
+    if (tid < kBins / 8) {
+#pragma unroll
+      for (int r = 0; r < CTAS; ++r) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int* from = bin + kBins - 8 * tid - 4 - 4 * h;
+          const int4 v = CTAS > 1 ? peer_words(from, r) : *reinterpret_cast<const int4*>(from);
+          sum[4 * h] += v.w, sum[4 * h + 1] += v.z, sum[4 * h + 2] += v.y, sum[4 * h + 3] += v.x;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) mine += sum[e];
+    }
+    int upto = mine;  // keys in this thread's bins and above, of those that this pass looks at
+    if (tid < kBins / 8) {
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int z = __shfl_up_sync(0xffffffffu, upto, d);
+        if ((tid & 31) >= d) upto += z;
+      }
+      if ((tid & 31) == 31) s_warp[0][tid >> 5] = upto;
     }
     __syncthreads();
-    // Thread t has the bins 2047 - 2 t and 2046 - 2 t: from the top.
-    const int hi = s_bin[kBins - 1 - 2 * tid], lo = s_bin[kBins - 2 - 2 * tid];
-    int all;
-    const int before = above + block_scan(hi + lo, s_warp, all);
-    if (before < wanted && before + hi + lo >= wanted) {
-      const bool first = before + hi >= wanted;
-      s_found = first ? kBins - 1 - 2 * tid : kBins - 2 - 2 * tid;
-      s_above = first ? before : before + hi;
+    if (tid < kBins / 8) {
+      upto += above - mine;
+      for (int w = 0; w < tid >> 5; ++w) upto += s_warp[0][w];
+      if (upto < wanted && upto + mine >= wanted) {
+        int e = 0;
+        while (upto + sum[0] < wanted) {  // shifts, so that the sums stay in registers
+          upto += sum[0];
+          ++e;
+#pragma unroll
+          for (int k = 0; k < 7; ++k) sum[k] = sum[k + 1];
+        }
+        s_found = kBins - 1 - 8 * tid - e;
+        s_above = upto;
+      }
     }
     __syncthreads();
     prefix = prefix << bits | static_cast<uint32_t>(s_found);
     above = s_above;
-    __syncthreads();
   }
   const int ties = wanted - above;  // of the keys equal to `prefix` the first ones
 
-  // ---- the list, four neighbouring tokens a thread at a time
+  // ---- the list: the keys above and equal to it in the CTAs before this one, then in the threads before
+  if (tid < 2) s_count[tid] = 0;
+  __syncthreads();
   int done_above = 0, done_ties = 0;
-  for (int i0 = 0; i0 < others; i0 += 4 * kSelectThreads) {
-    const int first = i0 + 4 * tid;
+  if constexpr (CTAS > 1) {
     int larger = 0, equal = 0;
-    uint32_t k[4];
+    visit([&](int i, const uint32_t (&k)[4]) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      k[e] = 0;
-      if (first + e < others) {
-        k[e] = key_at(first + e);
-        larger += k[e] > prefix;
-        equal += k[e] == prefix;
+      for (int e = 0; e < 4; ++e)
+        if (i + e < end) {
+          larger += k[e] > prefix;
+          equal += k[e] == prefix;
+        }
+    });
+    larger = __reduce_add_sync(0xffffffffu, larger);
+    equal = __reduce_add_sync(0xffffffffu, equal);
+    if ((tid & 31) == 0) {
+      atomicAdd(&s_count[0], larger);
+      atomicAdd(&s_count[1], equal);
+    }
+    meet();
+#pragma unroll
+    for (int r = 0; r < CTAS; ++r) {
+      const int4 v = peer_words(s_count, r);
+      if (r < rank) {
+        done_above += v.x;
+        done_ties += v.y;
       }
     }
-    int all;
-    const int scan = block_scan(larger | equal << 16, s_warp, all);  // at most 4096 each
-    int at_above = done_above + (scan & 0xffff), at_ties = done_ties + (scan >> 16);
+    __syncwarp();
+    cluster_arrive();  // no CTA ends while another one reads its shared memory
+  }
+  for (int i0 = begin; i0 < end; i0 += kRounds * kRoundKeys) {
+    int count[kRounds], all[kRounds];  // larger ones in the lower half, equal ones in the upper half: at most 4096 each
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (first + e < others) {
-        const bool is_tie = k[e] == prefix;
-        if (k[e] > prefix || (is_tie && at_ties < ties)) kept[at_above + min(at_ties, ties)] = first + e;
-        at_above += k[e] > prefix;
-        at_ties += is_tie;
-      }
-    done_above += all & 0xffff;
-    done_ties += all >> 16;
-    if (done_above == above && done_ties >= ties) break;
+    for (int r = 0; r < kRounds; ++r) {
+      const int i = i0 + r * kRoundKeys + 4 * tid;
+      count[r] = 0;
+      if (!held && i < end) read(i, key[r]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (i + e < end) count[r] += (key[r][e] > prefix ? 1 : 0) + (key[r][e] == prefix ? 1 << 16 : 0);
+    }
+    block_scan(count, all, min(kRounds, (end - i0 + kRoundKeys - 1) / kRoundKeys), s_warp);
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+      const int i = i0 + r * kRoundKeys + 4 * tid;
+      int at_above = done_above + (count[r] & 0xffff), at_ties = done_ties + (count[r] >> 16);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (i + e < end) {
+          const bool larger = key[r][e] > prefix, tie = key[r][e] == prefix;
+          if (larger || (tie && at_ties < ties)) kept[at_above + min(at_ties, ties)] = i + e;
+          at_above += larger;
+          at_ties += tie;
+        }
+      done_above += all[r] & 0xffff;
+      done_ties += all[r] >> 16;
+    }
+  }
+  if constexpr (CTAS > 1) {
+    __syncwarp();
+    cluster_wait();
   }
 }
 
-constexpr int kMoveThreads = 256, kMoveRows = 4;  // rows a thread has in flight
+constexpr int kMoveThreads = 256;
 
 // PIECES: 16-byte pieces of a row where they are known, 0: any number.
 template <int PIECES>
-__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_constant__ EvictParams p) {
+__global__ void __launch_bounds__(kMoveThreads, 8) evict_move_kernel(const __grid_constant__ EvictParams p) {
   early_wait();
   early_trigger();
   const int pieces = PIECES > 0 ? PIECES : p.head_dim / 8, per_pass = kMoveThreads / pieces;  // rows at a time
@@ -173,38 +315,23 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
   const int n = p.seqlens_out[b];
   if (row_in >= per_pass) return;
   const int32_t* kept = p.kept + static_cast<int64_t>(blockIdx.x) * p.budget;
-  const int64_t step = static_cast<int64_t>(gridDim.y) * per_pass * kMoveRows;
-  for (int64_t j0 = static_cast<int64_t>(blockIdx.y) * per_pass * kMoveRows + row_in; j0 < n; j0 += step) {
-    int from[kMoveRows];
-#pragma unroll
-    for (int u = 0; u < kMoveRows; ++u) from[u] = j0 + u * per_pass < n ? kept[j0 + u * per_pass] : -1;
-    uint4 kw[kMoveRows], vw[kMoveRows];
-    float mw[kMoveRows];
-    int64_t to_page[kMoveRows];
-#pragma unroll
-    for (int u = 0; u < kMoveRows; ++u) {
-      to_page[u] = -1;
-      if (from[u] < 0) continue;
-      const int page = p.from.page_of(b, from[u]);
-      const int to = p.to.page_of(b, static_cast<int>(j0) + u * per_pass);
-      if (page < 0 || to < 0) {
-        if (p.status != nullptr) atomicCAS(p.status, 0, static_cast<int>(kPagedBadPage));
-        continue;
-      }
-      to_page[u] = to;
-      const int row = p.from.page_size.mod(from[u]);
-      kw[u] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.k) + page * p.ks.outer + row * p.ks.row + hk * p.ks.head + piece * 8);
-      vw[u] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.v) + page * p.vs.outer + row * p.vs.row + hk * p.vs.head + piece * 8);
-      if (piece == 0) mw[u] = p.mass[(static_cast<int64_t>(page) * p.heads_k + hk) * p.from.page_size.d + row];
+  const int64_t step = static_cast<int64_t>(gridDim.y) * per_pass;
+  for (int64_t j = static_cast<int64_t>(blockIdx.y) * per_pass + row_in; j < n; j += step) {
+    const int from = kept[j];
+    const int page = p.from.page_of(b, from), to = p.to.page_of(b, static_cast<int>(j));
+    if (page < 0 || to < 0) {
+      if (p.status != nullptr) atomicCAS(p.status, 0, static_cast<int>(kPagedBadPage));
+      continue;
     }
-#pragma unroll
-    for (int u = 0; u < kMoveRows; ++u) {
-      if (to_page[u] < 0) continue;
-      const int row = p.from.page_size.mod(static_cast<int>(j0) + u * per_pass);
-      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.k) + to_page[u] * p.ks.outer + row * p.ks.row + hk * p.ks.head + piece * 8) = kw[u];
-      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.v) + to_page[u] * p.vs.outer + row * p.vs.row + hk * p.vs.head + piece * 8) = vw[u];
-      if (piece == 0) p.mass[(to_page[u] * p.heads_k + hk) * p.from.page_size.d + row] = mw[u];
-    }
+    const int row = p.from.page_size.mod(from), to_row = p.from.page_size.mod(static_cast<int>(j));
+    uint16_t *k = static_cast<uint16_t*>(p.k) + hk * p.ks.head + piece * 8, *v = static_cast<uint16_t*>(p.v) + hk * p.vs.head + piece * 8;
+    const uint4 kw = *reinterpret_cast<const uint4*>(k + page * p.ks.outer + row * p.ks.row);
+    const uint4 vw = *reinterpret_cast<const uint4*>(v + page * p.vs.outer + row * p.vs.row);
+    const int64_t at = static_cast<int64_t>(page) * p.heads_k + hk, to_at = static_cast<int64_t>(to) * p.heads_k + hk;
+    const float w = piece == 0 ? p.mass[at * p.from.page_size.d + row] : 0.f;
+    *reinterpret_cast<uint4*>(k + to * p.ks.outer + to_row * p.ks.row) = kw;
+    *reinterpret_cast<uint4*>(v + to * p.vs.outer + to_row * p.vs.row) = vw;
+    if (piece == 0) p.mass[to_at * p.from.page_size.d + to_row] = w;
   }
 }
 
@@ -212,17 +339,9 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
 
 namespace {
 
-template <bool HELD>
-cudaError_t launch_select(const EvictParams& p, size_t smem, cudaStream_t stream) {
-  static bool configured[64] = {};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev >= 0 && dev < 64 && !configured[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(evict_select_kernel<HELD>, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeld * 4);
-    if (e != cudaSuccess) return e;
-    configured[dev] = true;
-  }
-  return launch_grid(true, evict_select_kernel<HELD>, dim3(p.batch * p.heads_k), kSelectThreads, smem, stream, p);
+template <int CTAS>
+cudaError_t launch_select(const EvictParams& p, cudaStream_t stream) {
+  return launch_clusters(CTAS, evict_select_kernel<CTAS>, dim3(static_cast<unsigned>(p.batch * p.heads_k) * CTAS), kSelectThreads, 0, stream, p);
 }
 
 }  // namespace
@@ -230,9 +349,14 @@ cudaError_t launch_select(const EvictParams& p, size_t smem, cudaStream_t stream
 cudaError_t launch_paged_evict(const EvictParams& p, int sm_count, cudaStream_t stream) {
   const int units = p.batch * p.heads_k;
   const int64_t most = p.from.capacity();
-  cudaError_t e = most <= kHeld ? launch_select<true>(p, static_cast<size_t>(most) * 4, stream) : launch_select<false>(p, kHeld * 4, stream);
+  // Clusters where there are SMs for them and more than 8192 keys for a CTA: their barriers and the exchange take longer than that many
+  // keys. us a call of B2 Hk8 from 4096 tokens with 1, 2, 4, 8 CTAs: 16.3, 19.2, 20.9, 39.8; of B16 Hk4 from 16384: 93.0, 92.9, 106.5,
+  // 164; of B1 Hk8 from 131072: 226, 183, 147, 123.
+  const int64_t ctas = std::min<int64_t>((most + 8191) / 8192, sm_count / units);
+  cudaError_t e = ctas >= 8 ? launch_select<8>(p, stream) : ctas >= 4 ? launch_select<4>(p, stream) : ctas >= 2 ? launch_select<2>(p, stream)
+                                                                                                             : launch_select<1>(p, stream);
   if (e != cudaSuccess) return e;
-  const int rows = kMoveThreads / (p.head_dim / 8) * kMoveRows;
+  const int rows = kMoveThreads / (p.head_dim / 8);
   const int64_t blocks = (static_cast<int64_t>(p.budget) + rows - 1) / rows, fill = (64 * static_cast<int64_t>(sm_count) + units - 1) / units;
   const dim3 grid(units, static_cast<unsigned>(blocks < fill ? blocks : fill));
   if (p.head_dim == 128) return launch_grid(true, evict_move_kernel<16>, grid, kMoveThreads, 0, stream, p);
