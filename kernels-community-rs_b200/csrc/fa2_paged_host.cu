@@ -153,7 +153,7 @@ int plan_fwd(const fa2_paged_fwd_args* a, int sm_count, FwdPlan* f) {
   const int64_t capacity = std::min<int64_t>(static_cast<int64_t>(c->max_pages) * c->page_size, kMostRows);
   f->most_keys = static_cast<int>(a->max_seqlen_k > 0 ? std::min<int64_t>(a->max_seqlen_k, capacity) : capacity);
   f->rows = a->seqlen_q * (a->heads / c->heads_k);
-  const int unit_rows = fa2::paged_unit_rows(c->head_dim, f->rows);
+  const int unit_rows = fa2::paged_unit_rows(f->rows);
   f->row_tiles = (f->rows + unit_rows - 1) / unit_rows;
   const int64_t most_tiles = static_cast<int64_t>(c->batch) * c->heads_k * f->row_tiles * ((f->most_keys + static_cast<int64_t>(fa2::kPagedTile) - 1) / fa2::kPagedTile);
   f->grid = static_cast<int>(std::min<int64_t>(sm_count, (most_tiles + fa2::kPagedMinShare - 1) / fa2::kPagedMinShare));

@@ -87,12 +87,10 @@ cudaError_t launch_rotary(const RotaryParams& p, bool bf16, bool append, bool ve
 constexpr int kPagedMaxRows = 128;   // query rows per kv head
 constexpr int kPagedTile = 16;       // keys of a tile
 constexpr int kPagedMinShare = 4;    // tiles of a CTA's share at least, where there are that many
-// Query rows of a unit: what the accumulators of 64-column parts leave registers for.
-inline int paged_unit_rows(int head_dim, int rows) { return rows <= 8 ? 8 : rows <= 16 || head_dim > 128 ? 16 : 32; }
+// Query rows of a unit.
+inline int paged_unit_rows(int rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : 32; }
 // Floats of a partial result: O of a unit's rows, their maxima and sums.
-inline int64_t paged_part_floats(int head_dim, int rows) {
-  return paged_unit_rows(head_dim, rows) * (static_cast<int64_t>((head_dim + 63) / 64 * 64) + 2);
-}
+inline int64_t paged_part_floats(int head_dim, int rows) { return paged_unit_rows(rows) * (static_cast<int64_t>((head_dim + 63) / 64 * 64) + 2); }
 cudaError_t launch_fwd_paged(const PagedParams& p, int grid, int sm_count, bool bf16, cudaStream_t stream);
 
 cudaError_t launch_paged_evict(const EvictParams& p, int sm_count, cudaStream_t stream);

@@ -29,23 +29,25 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-template <int A, int NT>  // 64-column parts of the head dim; 8-row tiles of a unit
+// A: 64-column parts of the head dim. NT: 8-row tiles of a warp. TEAM: warps that work on the same keys, each on its own rows.
+template <int A, int NT, int TEAM>
 struct Cfg {
   static constexpr int D = A * 64;
-  static constexpr int kRows = 8 * NT;
-  static constexpr int kWarps = A == 1 ? (NT == 1 ? 14 : NT == 2 ? 12 : 8) : A == 2 ? (NT == 1 ? 10 : 8) : A == 3 ? 7 : 5;
+  static constexpr int kRows = 8 * NT * TEAM;
+  static constexpr int kWarps = A == 1 ? (NT == 1 ? 14 : NT == 2 ? 12 : 8) : A == 2 ? (NT == 1 ? 10 : 8) : A == 3 ? (TEAM == 1 ? 7 : 8) : (TEAM == 1 ? 5 : 8);
+  static constexpr int kTeams = kWarps / TEAM;
   static constexpr int kThreads = kWarps * 32;
   // A tile's 16 rows of K, then of V: 64 columns at a time, rows of 128 bytes whose 16-byte pieces are swizzled by the row.
   static constexpr int kPart = 2048;
-  static constexpr int kVOff = A * kPart, kStageBytes = 2 * A * kPart;  // of a warp
-  static constexpr int kStages = A == 1 ? (NT == 4 ? 5 : 3) : 2;
-  static constexpr int kQueueBytes = kWarps * kStages * kStageBytes;
+  static constexpr int kVOff = A * kPart, kStageBytes = 2 * A * kPart;  // of a team
+  static constexpr int kStages = A == 1 ? (NT < 4 ? 3 : 5) : A == 3 && TEAM > 1 ? 3 : 2;
+  static constexpr int kQueueBytes = kTeams * kStages * kStageBytes;
   static constexpr bool kQInRegs = A * NT <= 4;          // else its fragments stay in shared memory
-  static constexpr int kQBytes = kQInRegs ? 0 : NT * A * 2 * 512;
+  static constexpr int kQBytes = kQInRegs ? 0 : TEAM * NT * A * 2 * 512;
   static constexpr int kRowFloats = D + 4;               // a row of a warp's O when the warps' parts become one, 8 rows at a time
   static constexpr int kPartOff = kQueueBytes + kQBytes, kPartBytes = kWarps * 8 * kRowFloats * 4;
   static constexpr int kBarOff = kPartOff + kPartBytes;
-  static constexpr int kSmemBytes = kBarOff + kWarps * kStages * 8;
+  static constexpr int kSmemBytes = kBarOff + kTeams * kStages * 8;
   static_assert(kSmemBytes <= 227 * 1024 - 6144, "shared memory");
 };
 
@@ -105,7 +107,7 @@ __device__ __forceinline__ uint32_t transposed(uint32_t w) {
   return r;
 }
 
-// A unit: up to 8 NT query rows of a kv head of a sequence, and the part of its 16-key tiles that a share has.
+// A unit: up to 8 NT TEAM query rows of a kv head of a sequence, and the part of its 16-key tiles that a share has.
 struct Segment {
   int b, hk, rt;       // sequence, kv head, row tile
   int unit;            // within the sequence
@@ -131,10 +133,10 @@ __device__ __forceinline__ void store_row(const PagedParams& p, int b, int hk, i
 
 // TILED: pages are whole tiles, so that a tile is one TMA box for each 64 columns of K and of V. Otherwise its rows lie in two or more
 // pages, and are copied 16 bytes at a time.
-template <int A, int NT, bool BF16, bool TILED>
-__global__ void __launch_bounds__((Cfg<A, NT>::kThreads), 1) fwd_paged_kernel(const __grid_constant__ PagedParams p) {
-  using C = Cfg<A, NT>;
-  constexpr int D = C::D, W = C::kWarps, R = C::kRows, kStages = C::kStages;
+template <int A, int NT, int TEAM, bool BF16, bool TILED>
+__global__ void __launch_bounds__((Cfg<A, NT, TEAM>::kThreads), 1) fwd_paged_kernel(const __grid_constant__ PagedParams p) {
+  using C = Cfg<A, NT, TEAM>;
+  constexpr int D = C::D, W = C::kWarps, R = C::kRows, kStages = C::kStages, kTeams = C::kTeams;
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ int64_t s_sum[W];
   __shared__ int64_t s_before;        // tiles of the sequences before s_first
@@ -143,10 +145,11 @@ __global__ void __launch_bounds__((Cfg<A, NT>::kThreads), 1) fwd_paged_kernel(co
   __shared__ int s_abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t4 = lane & 3;
-  uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + C::kBarOff) + warp * kStages;  // this warp's
+  const int team = warp / TEAM, mate = warp - team * TEAM;  // its first warp starts the copies
+  uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + C::kBarOff) + team * kStages;  // this team's
   const WaitCtl ctl{&s_abort};
   if (tid == 0) s_abort = 0;
-  if (lane < kStages) mbar_init(&bars[lane], TILED ? 1 : 32);
+  if (mate == 0 && lane < kStages) mbar_init(&bars[lane], TILED ? 1 : 32);
   mbar_fence_init();
   if (TILED && tid == 0) {
     tma_prefetch_desc(&p.tm_k);
@@ -268,7 +271,7 @@ __global__ void __launch_bounds__((Cfg<A, NT>::kThreads), 1) fwd_paged_kernel(co
   }
   open_unit(lo);
 
-  const uint32_t queue = smem_u32(smem) + warp * (kStages * C::kStageBytes);
+  const uint32_t queue = smem_u32(smem) + team * (kStages * C::kStageBytes);
   const uint32_t q_smem = smem_u32(smem) + C::kQueueBytes + lane * 16;
   const float inv_cap = p.softcap > 0.f ? p.scale / p.softcap : 0.f;
   const float cap_l2 = p.softcap * kLog2e;
@@ -290,7 +293,7 @@ __global__ void __launch_bounds__((Cfg<A, NT>::kThreads), 1) fwd_paged_kernel(co
     if (j >= seg.j1 || key >= seg.end_all || (!TILED && key < seg.begin_all)) return -1;
     return p.table.pages[seg.b * p.table.stride + p.table.page_size.div(key)];
   };
-  // Starts the copies of tile j into a stage that every lane has read, and returns a bit for each of its keys that some row sees.
+  // Starts the copies of tile j into a stage that all lanes of the team have read, and returns a bit for each of its keys that some row sees.
   auto issue = [&](int j, int page, int to_stage) {
     const int key0 = first_key(j);
     if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(p.table.num_pages)) {
@@ -302,7 +305,7 @@ __global__ void __launch_bounds__((Cfg<A, NT>::kThreads), 1) fwd_paged_kernel(co
     uint32_t seen;
     if constexpr (TILED) {
       seen = page < 0 ? 0u : bit_range(seg.begin_all - key0, min(seg.end_all - key0, 16));
-      if (elect_one()) {
+      if (mate == 0 && elect_one()) {
         mbar_expect_tx(&bars[to_stage], page < 0 ? 0 : C::kStageBytes);
         if (page >= 0) {
           const int row = p.table.page_size.mod(key0);
@@ -319,17 +322,19 @@ __global__ void __launch_bounds__((Cfg<A, NT>::kThreads), 1) fwd_paged_kernel(co
       const int row = p.table.page_size.mod(key0 + (lane & 15));
       const int64_t k_row = page < 0 ? 0 : page * p.ks.outer + row * p.ks.row;
       const int64_t v_row = page < 0 ? 0 : page * p.vs.outer + row * p.vs.row;
-      // Neighbouring lanes take neighbouring pieces of a row; what is not there is zero.
+      if (mate == 0) {
+        // Neighbouring lanes take neighbouring pieces of a row; what is not there is zero.
 #pragma unroll
-      for (int i = 0; i < A * 4; ++i) {
-        const int r = (lane + 32 * i) / (A * 8), c = lane + 32 * i - r * (A * 8);
-        const bool there = (seen >> r & 1) && c * 8 < p.head_dim;
-        const uint32_t to = at + (c >> 3) * C::kPart + r * 128 + (((c ^ r) & 7) << 4);
-        const int64_t k_from = __shfl_sync(0xffffffffu, k_row, r) + c * 8, v_from = __shfl_sync(0xffffffffu, v_row, r) + c * 8;
-        copy16(to, static_cast<const uint16_t*>(p.k) + seg.hk * p.ks.head + (there ? k_from : 0), there);
-        copy16(to + C::kVOff, static_cast<const uint16_t*>(p.v) + seg.hk * p.vs.head + (there ? v_from : 0), there);
+        for (int i = 0; i < A * 4; ++i) {
+          const int r = (lane + 32 * i) / (A * 8), c = lane + 32 * i - r * (A * 8);
+          const bool there = (seen >> r & 1) && c * 8 < p.head_dim;
+          const uint32_t to = at + (c >> 3) * C::kPart + r * 128 + (((c ^ r) & 7) << 4);
+          const int64_t k_from = __shfl_sync(0xffffffffu, k_row, r) + c * 8, v_from = __shfl_sync(0xffffffffu, v_row, r) + c * 8;
+          copy16(to, static_cast<const uint16_t*>(p.k) + seg.hk * p.ks.head + (there ? k_from : 0), there);
+          copy16(to + C::kVOff, static_cast<const uint16_t*>(p.v) + seg.hk * p.vs.head + (there ? v_from : 0), there);
+        }
+        copies_arrive(&bars[to_stage]);
       }
-      copies_arrive(&bars[to_stage]);
     }
     return seen;
   };
@@ -339,12 +344,12 @@ __global__ void __launch_bounds__((Cfg<A, NT>::kThreads), 1) fwd_paged_kernel(co
   auto fill = [&]() {
     int page[kStages];
 #pragma unroll
-    for (int i = 0; i < kStages; ++i) page[i] = look_up(seg.j0 + warp + i * W);
-    next_page = look_up(seg.j0 + warp + kStages * W);
+    for (int i = 0; i < kStages; ++i) page[i] = look_up(seg.j0 + team + i * kTeams);
+    next_page = look_up(seg.j0 + team + kStages * kTeams);
 #pragma unroll
     for (int i = 0; i < kStages; ++i) {
       seen_of[i] = 0;
-      if (seg.j0 + warp + i * W < seg.j1) seen_of[i] = issue(seg.j0 + warp + i * W, page[i], stage + i < kStages ? stage + i : stage + i - kStages);
+      if (seg.j0 + team + i * kTeams < seg.j1) seen_of[i] = issue(seg.j0 + team + i * kTeams, page[i], stage + i < kStages ? stage + i : stage + i - kStages);
     }
   };
   fill();
@@ -354,6 +359,7 @@ __global__ void __launch_bounds__((Cfg<A, NT>::kThreads), 1) fwd_paged_kernel(co
   for (bool more = true; more;) {
     const int row0 = seg.rt * R;
     const int rows = min(R, p.rows - row0);
+    const int my_row0 = row0 + 8 * NT * mate, my_rows = rows - 8 * NT * mate;  // this warp's; it may have none
     // Keys [same_lo, same_hi) are seen by every row of the call.
     const int same_hi = seg.length - p.seqlen_q + 1;
     const int same_lo = p.window < 0 ? 0 : seg.length - 1 - p.window;
@@ -365,8 +371,8 @@ __global__ void __launch_bounds__((Cfg<A, NT>::kThreads), 1) fwd_paged_kernel(co
     uint4 qf[C::kQInRegs ? NT * A * 2 : 1];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      if (!C::kQInRegs && n != warp) continue;  // every warp needs the same
-      const int r = row0 + 8 * n + g, q = p.group.div(r);
+      if (!C::kQInRegs && (n > 0 || warp >= TEAM * NT)) continue;  // in shared memory each tile is written by one warp
+      const int tile = C::kQInRegs ? mate * NT + n : warp, r = row0 + 8 * tile + g, q = p.group.div(r);
       const uint16_t* base = static_cast<const uint16_t*>(p.q) + seg.b * p.qs.outer + q * p.qs.row + (seg.hk * group + r - q * group) * p.qs.head;
 #pragma unroll
       for (int i = 0; i < A * 2; ++i) {
@@ -374,12 +380,12 @@ __global__ void __launch_bounds__((Cfg<A, NT>::kThreads), 1) fwd_paged_kernel(co
         uint4 w = make_uint4(0, 0, 0, 0);
         if (r < p.rows && e < p.head_dim) w = *reinterpret_cast<const uint4*>(base + e);
         if constexpr (C::kQInRegs) qf[n * (A * 2) + i] = w;
-        else sts16(q_smem + (n * (A * 2) + i) * 512, w);
+        else sts16(q_smem + (tile * (A * 2) + i) * 512, w);
       }
     }
     if constexpr (!C::kQInRegs) __syncthreads();
 
-    // Rows of this thread: row0 + 8 n + 2 t4 + e.
+    // Rows of this thread: my_row0 + 8 n + 2 t4 + e.
     float m[NT][2], l[NT][2];
     float o[A * 4][NT][4];
 #pragma unroll
@@ -390,7 +396,7 @@ __global__ void __launch_bounds__((Cfg<A, NT>::kThreads), 1) fwd_paged_kernel(co
       for (int i = 0; i < A * 4; ++i) o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.f;
     }
 
-    for (int j = seg.j0 + warp; j < seg.j1; j += W) {
+    for (int j = seg.j0 + team; j < seg.j1; j += kTeams) {
       warp_wait(&bars[stage], phase, ctl, kWaitPaged + 1);
       const uint32_t at = queue + stage * C::kStageBytes;
       const uint32_t seen = seen_of[0];
@@ -408,7 +414,7 @@ __global__ void __launch_bounds__((Cfg<A, NT>::kThreads), 1) fwd_paged_kernel(co
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           if constexpr (C::kQInRegs) b[n] = qf[n * (A * 2) + i];
-          else b[n] = lds16(q_smem + (n * (A * 2) + i) * 512);
+          else b[n] = lds16(q_smem + ((mate * NT + n) * (A * 2) + i) * 512);
         }
         // Neighbouring products have different sums.
 #pragma unroll
@@ -436,24 +442,25 @@ __global__ void __launch_bounds__((Cfg<A, NT>::kThreads), 1) fwd_paged_kernel(co
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int k = g + 8 * (e >> 1), q = p.group.div(row0 + 8 * n + 2 * t4 + (e & 1));
+            const int k = g + 8 * (e >> 1), q = p.group.div(my_row0 + 8 * n + 2 * t4 + (e & 1));
             if (!(seen >> k & 1) || key0 + k >= to(q) || key0 + k < from(q)) s[n][e] = -INFINITY;
           }
       }
       if (p.scores != nullptr) {
-        float* out = p.scores + ((static_cast<int64_t>(seg.b) * p.heads_k + seg.hk) * p.rows + row0 + 2 * t4) * p.score_stride + key0 + g;
+        float* out = p.scores + ((static_cast<int64_t>(seg.b) * p.heads_k + seg.hk) * p.rows + my_row0 + 2 * t4) * p.score_stride + key0 + g;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (8 * n + 2 * t4 + (e & 1) < rows) __stcg(out + (8 * n + (e & 1)) * p.score_stride + 8 * (e >> 1), s[n][e]);
+            if (8 * n + 2 * t4 + (e & 1) < my_rows) __stcg(out + (8 * n + (e & 1)) * p.score_stride + 8 * (e >> 1), s[n][e]);
       }
-      // ---- row maxima: the running ones hold until some score exceeds them
+      // ---- row maxima. The running ones hold until some score exceeds them by more than 8 (in the log2 domain): P is then at most 2^8,
+      // which costs neither of the two formats nor the fp32 sums any precision, and O is rarely rescaled.
       bool more = false;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) more = more || fmaxf(s[n][e], s[n][2 + e]) > m[n][e];
+        for (int e = 0; e < 2; ++e) more = more || fmaxf(s[n][e], s[n][2 + e]) > m[n][e] + 8.f;
       if (__any_sync(0xffffffffu, more)) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -530,7 +537,7 @@ __global__ void __launch_bounds__((Cfg<A, NT>::kThreads), 1) fwd_paged_kernel(co
         values(halves(seen >> (2 * t4)), halves(seen >> (2 * t4 + 8)), add_all);
       } else {
         // One query at a time, with the values that it does not see at zero, into the rows of that query alone.
-        for (int q = p.group.div(row0); q <= p.group.div(row0 + rows - 1); ++q) {
+        for (int q = p.group.div(my_row0); q <= p.group.div(my_row0 + max(min(my_rows, 8 * NT), 1) - 1); ++q) {
           const uint32_t sees = seen & bit_range(from(q) - key0, to(q) - key0);
           values(halves(sees >> (2 * t4)), halves(sees >> (2 * t4 + 8)), [&](int i, const uint32_t (&a)[4]) {
 #pragma unroll
@@ -540,7 +547,7 @@ __global__ void __launch_bounds__((Cfg<A, NT>::kThreads), 1) fwd_paged_kernel(co
               mma16816<BF16>(c, a, p_lo[n][0], p_lo[n][1]);
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                if (p.group.div(row0 + 8 * n + 2 * t4 + (e & 1)) == q) o[i][n][e] += c[e];
+                if (p.group.div(my_row0 + 8 * n + 2 * t4 + (e & 1)) == q) o[i][n][e] += c[e];
             }
           });
         }
@@ -549,9 +556,10 @@ __global__ void __launch_bounds__((Cfg<A, NT>::kThreads), 1) fwd_paged_kernel(co
 #pragma unroll
       for (int i = 0; i + 1 < kStages; ++i) seen_of[i] = seen_of[i + 1];
       __syncwarp();
-      if (j + kStages * W < seg.j1) {
-        seen_of[kStages - 1] = issue(j + kStages * W, next_page, stage);
-        next_page = look_up(j + (kStages + 1) * W);
+      if constexpr (TEAM > 1) asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(TEAM * 32) : "memory");
+      if (j + kStages * kTeams < seg.j1) {
+        seen_of[kStages - 1] = issue(j + kStages * kTeams, next_page, stage);
+        next_page = look_up(j + (kStages + 1) * kTeams);
       }
       if (++stage == kStages) {
         stage = 0;
@@ -581,7 +589,7 @@ __global__ void __launch_bounds__((Cfg<A, NT>::kThreads), 1) fwd_paged_kernel(co
     }
     float* const slot = p.partials + (2 * static_cast<int64_t>(blockIdx.x) + (done.j0 == 0 ? 1 : 0)) * kSlot;
     float* const parts = reinterpret_cast<float*>(smem + C::kPartOff);  // [warp][8 rows][D + 4]
-    const int warps = min(W, done.j1 - done.j0);  // those that had a tile
+    const int teams = min(kTeams, done.j1 - done.j0);  // those that had a tile
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       if (8 * n >= rows) break;
@@ -596,7 +604,7 @@ __global__ void __launch_bounds__((Cfg<A, NT>::kThreads), 1) fwd_paged_kernel(co
           s_m[warp][r] = m[n][e];
           s_l[warp][r] = x;
         }
-        if (warp < warps && 8 * n + r < rows) {
+        if (team < teams && 8 * n + r < my_rows) {
           float* row = parts + (warp * 8 + r) * C::kRowFloats + 8 * g;
 #pragma unroll
           for (int i = 0; i < A; ++i) {
@@ -606,14 +614,16 @@ __global__ void __launch_bounds__((Cfg<A, NT>::kThreads), 1) fwd_paged_kernel(co
         }
       }
       __syncthreads();
-      for (int i = tid; i < min(8, rows - 8 * n) * (D / 4); i += C::kThreads) {
-        const int r = i / (D / 4), col = i % (D / 4) * 4;
+      for (int i = tid; i < TEAM * 8 * (D / 4); i += C::kThreads) {
+        const int r = i / (D / 4) % 8, x = i / (D / 4) / 8, col = i % (D / 4) * 4;
+        const int row = 8 * (NT * x + n) + r;  // of the unit: row r of the n-th tile of the x-th warp of each team
+        if (row >= rows) continue;
         float top = -INFINITY;
-        for (int w = 0; w < warps; ++w) top = fmaxf(top, s_m[w][r]);
+        for (int w = x; w < teams * TEAM; w += TEAM) top = fmaxf(top, s_m[w][r]);
         float total = 0.f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-        for (int w = 0; w < warps; ++w) {
+        for (int w = x; w < teams * TEAM; w += TEAM) {
           const float f = part_scale(s_m[w][r], top);
           const float4 v = *reinterpret_cast<const float4*>(parts + (w * 8 + r) * C::kRowFloats + col);
           total += f * s_l[w][r];
@@ -623,12 +633,12 @@ __global__ void __launch_bounds__((Cfg<A, NT>::kThreads), 1) fwd_paged_kernel(co
           acc.w += f * v.w;
         }
         if (whole) {
-          store_row<BF16>(p, done.b, done.hk, row0 + 8 * n + r, col, acc, top, total);
+          store_row<BF16>(p, done.b, done.hk, row0 + row, col, acc, top, total);
         } else {
-          __stcg(reinterpret_cast<float4*>(slot + (8 * n + r) * D + col), acc);
+          __stcg(reinterpret_cast<float4*>(slot + row * D + col), acc);
           if (col == 0) {
-            __stcg(slot + R * D + 8 * n + r, top);
-            __stcg(slot + R * D + R + 8 * n + r, total);
+            __stcg(slot + R * D + row, top);
+            __stcg(slot + R * D + R + row, total);
           }
         }
       }
@@ -780,33 +790,34 @@ __global__ void __launch_bounds__(kTailThreads) paged_tail_kernel(const __grid_c
   }
 }
 
-template <int A, int NT, bool BF16, bool TILED>
+template <int A, int NT, int TEAM, bool BF16, bool TILED>
 cudaError_t launch_one(const PagedParams& p, int grid, cudaStream_t stream) {
-  using C = Cfg<A, NT>;
+  using C = Cfg<A, NT, TEAM>;
   static bool configured[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 0 && dev < 64 && !configured[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(fwd_paged_kernel<A, NT, BF16, TILED>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+    cudaError_t e = cudaFuncSetAttribute(fwd_paged_kernel<A, NT, TEAM, BF16, TILED>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
     if (e != cudaSuccess) return e;
     configured[dev] = true;
   }
-  return launch_grid(true, fwd_paged_kernel<A, NT, BF16, TILED>, dim3(grid), C::kThreads, C::kSmemBytes, stream, p);
+  return launch_grid(true, fwd_paged_kernel<A, NT, TEAM, BF16, TILED>, dim3(grid), C::kThreads, C::kSmemBytes, stream, p);
 }
 
-template <int A, int NT, bool BF16>
+template <int A, int NT, int TEAM, bool BF16>
 cudaError_t pick_copies(const PagedParams& p, int grid, cudaStream_t stream) {
-  return p.tiled ? launch_one<A, NT, BF16, true>(p, grid, stream) : launch_one<A, NT, BF16, false>(p, grid, stream);
+  return p.tiled ? launch_one<A, NT, TEAM, BF16, true>(p, grid, stream) : launch_one<A, NT, TEAM, BF16, false>(p, grid, stream);
 }
 
 template <int A, bool BF16>
 cudaError_t pick_rows(const PagedParams& p, int grid, cudaStream_t stream) {
-  const int rows = paged_unit_rows(p.head_dim, p.rows);
-  if (rows == 8) return pick_copies<A, 1, BF16>(p, grid, stream);
-  if constexpr (A <= 2) {
-    if (rows == 32) return pick_copies<A, 4, BF16>(p, grid, stream);
-  }
-  return pick_copies<A, 2, BF16>(p, grid, stream);
+  const int rows = paged_unit_rows(p.rows);
+  if (rows == 8) return pick_copies<A, 1, 1, BF16>(p, grid, stream);
+  if (rows == 16) return pick_copies<A, 2, 1, BF16>(p, grid, stream);
+  // A warp has registers for 32 rows of 128 columns; of more columns two warps take 16 rows each of the same keys. (Where one can, two
+  // are slower: 32 rows against 131072 keys of 8 heads at D128 134 us, with one 120.)
+  if constexpr (A <= 2) return pick_copies<A, 4, 1, BF16>(p, grid, stream);
+  else return pick_copies<A, 2, 2, BF16>(p, grid, stream);
 }
 
 template <bool BF16>
@@ -823,7 +834,7 @@ cudaError_t launch_fwd_paged(const PagedParams& p, int grid, int sm_count, bool 
   if (p.rows <= 0 || p.rows > kPagedMaxRows || p.head_dim <= 0 || p.head_dim > 256 || grid <= 0) return cudaErrorInvalidValue;
   const cudaError_t e = bf16 ? pick_dim<true>(p, grid, stream) : pick_dim<false>(p, grid, stream);
   if (e != cudaSuccess) return e;
-  const int d = (p.head_dim + 63) / 64 * 64, unit_rows = paged_unit_rows(p.head_dim, p.rows), joins = grid * (unit_rows / 8);
+  const int d = (p.head_dim + 63) / 64 * 64, unit_rows = paged_unit_rows(p.rows), joins = grid * (unit_rows / 8);
   // Blocks for every key that there can be, but no more than fill the GPU a few times over: lengths are known on the device only.
   const int64_t units = static_cast<int64_t>(p.batch) * p.heads_k, keys = 4 * kTailThreads;
   const int64_t every = (static_cast<int64_t>(p.most_keys) + 3 + keys - 1) / keys, fill = (32 * static_cast<int64_t>(sm_count) + units - 1) / units;
