@@ -7,6 +7,7 @@
 #include <climits>
 #include <cmath>
 #include <cstring>
+#include <initializer_list>
 
 namespace {
 
@@ -29,6 +30,12 @@ bool addressable(const void* ptr, const int64_t* stride) {
   return true;
 }
 
+bool aligned4(std::initializer_list<const void*> pointers) {
+  for (const void* p : pointers)
+    if (reinterpret_cast<uintptr_t>(p) % 4 != 0) return false;
+  return true;
+}
+
 int check_types(int dtype, int head_dim) {
   if (dtype != FA2_F16 && dtype != FA2_BF16) return fail(FA2_E_TYPE, "tensors must be float16 or bfloat16");
   if (head_dim < 8 || head_dim > 256 || head_dim % 8 != 0)
@@ -48,6 +55,7 @@ int check_cache(const fa2_paged_cache* c) {
   if (static_cast<int64_t>(c->batch) * c->heads_k > kMostRows) return fail(FA2_E_VALUE, "batch * heads_k must be below %d", kMostRows);
   if (c->k == nullptr || c->v == nullptr || c->block_table == nullptr || c->seqlens_k == nullptr)
     return fail(FA2_E_VALUE, "k, v, block_table and seqlens_k must be non-null");
+  if (!aligned4({c->attn_mass, c->block_table, c->seqlens_k})) return fail(FA2_E_VALUE, "attn_mass, block_table and seqlens_k must be 4-byte aligned");
   for (int i = 0; i < 3; ++i)
     if (c->k_stride[i] < 0 || c->v_stride[i] < 0) return fail(FA2_E_VALUE, "strides of k and v must not be negative");
   if (!addressable(c->k, c->k_stride) || !addressable(c->v, c->v_stride))
@@ -223,6 +231,7 @@ int fa2_paged_append(const fa2_paged_append_args* args, void* stream) {
   if (args->cu_seqlens == nullptr && t->batch != c->batch) return fail(FA2_E_VALUE, "the new tokens must have the cache's batch");
   if (p.tokens == 0) return FA2_OK;
   if (args->v == nullptr || reinterpret_cast<uintptr_t>(args->v) % 2) return fail(FA2_E_VALUE, "v must be non-null and aligned to its elements");
+  if (!aligned4({args->cu_seqlens, args->seqlens_new})) return fail(FA2_E_VALUE, "cu_seqlens and seqlens_new must be 4-byte aligned");
   const DeviceScope scope(c->k);
   Runtime* rt = nullptr;
   if ((rc = get_runtime(scope.device(), &rt)) != FA2_OK) return rc;
@@ -257,6 +266,7 @@ int fa2_paged_fwd(const fa2_paged_fwd_args* args, void* workspace, int64_t works
   if (args->seqlen_q == 0) return FA2_OK;
   const fa2_paged_cache* c = args->cache;
   if (args->q == nullptr || args->out == nullptr || args->lse == nullptr) return fail(FA2_E_VALUE, "q, out and lse must be non-null");
+  if (!aligned4({args->lse})) return fail(FA2_E_VALUE, "lse must be 4-byte aligned");
   if (!addressable(args->q, args->q_stride) || !addressable(args->out, args->o_stride))
     return fail(FA2_E_VALUE, "q and out must be 16-byte aligned, with outer strides that are multiples of 8 elements");
   const DeviceScope scope(c->k);
@@ -277,7 +287,10 @@ int fa2_paged_fwd(const fa2_paged_fwd_args* args, void* workspace, int64_t works
   p.vs = strides(c->v_stride);
   p.os = strides(args->o_stride);
   p.table = table_of(c);
-  p.tiled = c->page_size % fa2::kPagedTile == 0;
+  // A tensor map needs strides other than zero; heads or pages that share their memory are copied like pages of other sizes.
+  const bool apart = (c->heads_k == 1 || (c->k_stride[2] > 0 && c->v_stride[2] > 0)) && (c->page_size == 1 || (c->k_stride[1] > 0 && c->v_stride[1] > 0)) &&
+                     (c->num_pages == 1 || (c->k_stride[0] > 0 && c->v_stride[0] > 0));
+  p.tiled = c->page_size % fa2::kPagedTile == 0 && apart;
   if (p.tiled) {
     const bool wide = c->head_dim * 2 % 256 == 0;
     if ((rc = fa2::make_map(&p.tm_k, c->k, c->dtype, 2, c->head_dim, c->heads_k, c->page_size, c->num_pages, c->k_stride[2], c->k_stride[1],
@@ -325,10 +338,11 @@ int fa2_paged_evict(const fa2_paged_evict_args* args, void* stream) {
   const fa2_paged_cache* c = args->cache;
   if (args->reserved != 0) return fail(FA2_E_VALUE, "reserved must be 0");
   if (c->attn_mass == nullptr) return fail(FA2_E_VALUE, "attn_mass is null");
-  if (args->budget < 1 || args->recent < 0 || args->recent > args->budget)
-    return fail(FA2_E_VALUE, "budget must be positive and recent in 0..=budget, got %d and %d", args->budget, args->recent);
+  if (args->budget < 1 || args->budget > kMostRows || args->recent < 0 || args->recent > args->budget)
+    return fail(FA2_E_VALUE, "budget must be in 1..=%d and recent in 0..=budget, got %d and %d", kMostRows, args->budget, args->recent);
   if (args->dst_block_table == nullptr || args->seqlens_out == nullptr || args->kept == nullptr || args->dst_max_pages <= 0)
     return fail(FA2_E_VALUE, "dst_block_table, seqlens_out and kept must be non-null, dst_max_pages positive");
+  if (!aligned4({args->dst_block_table, args->seqlens_out, args->kept})) return fail(FA2_E_VALUE, "dst_block_table, seqlens_out and kept must be 4-byte aligned");
   const DeviceScope scope(c->k);
   Runtime* rt = nullptr;
   if ((rc = get_runtime(scope.device(), &rt)) != FA2_OK) return rc;

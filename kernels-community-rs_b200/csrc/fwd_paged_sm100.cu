@@ -2,23 +2,32 @@
 //
 //   O = softmax(f(Q K^T)) V over the keys of the sequence's pages, f the scale and the soft cap; running maximum m and sum l.
 //
-// What bounds it: reading K and V once (4 D bytes a key and kv head, 4 D operations for each of them and each query row: 1 to 16
-// operations a byte). So:
+// What bounds it: reading K and V once, 4 D bytes a key and kv head; 4 D operations for each of them and each query row, 1 to 32
+// operations a byte. So:
 //
-//   * The query rows of a kv head (row r = query r / group, head r % group) are the M of one product, 16 at a time.
-//   * The lengths are on the device. Every CTA, one per SM, adds up the sequences' key tiles and takes an equal share of the list
-//     of all (sequence, kv head, key tile); a share may begin and end inside a unit. A CTA leaves its part of a unit that it does
-//     not cover alone in the workspace, and a second kernel, which waits beside the first, adds the parts up (and the keys' weights).
-//   * A thread's copies are its own. mma.sync takes B fragments whose k index may be permuted freely as long as A's is alike, and
-//     n is only a name; so lane (g, t) = (lane / 4, lane % 4) takes 16-byte pieces t, t + 4, ... of key g's row as two k-steps of
-//     Q K^T, and pieces g, g + 8, ... of the rows of keys 2t, 2t + 1, 2t + 8, 2t + 9 as columns of P V. Every lane therefore reads
-//     from shared memory only what it copied there itself (cp.async): a queue per thread, without barriers between threads, with
-//     any page size, and free of bank conflicts because a copy's 32 pieces lie side by side. Each of the 8 (4) warps of a CTA
-//     walks its own keys, 16 at a time, with about 190 KB of copies in flight per SM.
-//   * P goes into P V as the sum of two 16-bit numbers, so that its rounding is 2^-16 (2^-21) instead of 2^-9 (2^-12) of it, and
-//     the output's error is its own rounding. The tensor cores are idle most of the time anyway.
-//   * Keys that no row sees are not read: their rows are zeroes and their scores -inf. Where some rows see a key and others do
-//     not, P's zero meets its value, and a value that is not finite would make a NaN of it: such values take a path of their own.
+//   * The query rows of a kv head (row r = query r / group, head r % group) share its K and V: up to 32 rows are one unit of work.
+//   * The lengths are on the device. Every CTA, one per SM, adds up the sequences' 16-key tiles and takes an equal share of the list
+//     of all (sequence, kv head, row tile, key tile); a share may begin and end inside a unit. A CTA leaves its part of a unit that it
+//     does not cover alone in the workspace, and a second kernel, which waits beside the first, adds the parts up (and the keys' weights).
+//   * Each warp walks key tiles of its own and keeps a queue of two or more of them in flight, 130 to 170 KB per SM: TMA boxes of 64
+//     columns where a tile lies in one page, else copies of 16 bytes by cp.async, of which an SM has only some 32 KB in flight. (One
+//     bulk copy for each row, for any page size, took 14 cycles a row: 18 B/clk per SM, where memory gives 29.) The queue goes on
+//     over the ends of units: the next unit's copies start before the warps' parts of the last one are added up.
+//   * The products are transposed, S^T = K Q^T and O^T = V^T P^T, by mma.sync m16n8k16: the keys (the columns of V) are the 16, 8
+//     query rows the 8, so that 8 rows, one token's heads in most models, waste nothing. Which d a k index means is free as long as
+//     K and Q agree, and so is which column of V a row of O^T is: a lane reads 16 bytes of shared memory at a time, and the
+//     pairs of keys that a fragment of V^T wants come from two such reads by byte permutes. P's fragments are transposed by movmatrix.
+//     (tcgen05 would multiply 128 rows at a time and hold P in another memory; 8 rows leave it nothing to win.)
+//   * P goes into P V as the sum of two 16-bit numbers, so that its rounding is 2^-16 (fp16: 2^-22) of it in place of 2^-8 (2^-11), and
+//     the output's error is its own rounding. mma.sync issues once in 16 cycles per scheduler here; up to 16 rows memory
+//     hides that, with 32 rows the products bound the call (96 of them for 16 keys). A value that is not finite gives a result that is
+//     not finite, though an infinity may become a NaN by the two products.
+//   * Keys that no row sees are not read or count as zero, whatever lies there. Where some rows see a key and others do not, P's
+//     zero meets its value, and a value that is not finite would make a NaN of it: such values take a path of their own.
+//
+// Measured (us a call, share of the measured copy rate): B1 H32/8 D128 8192 keys 15.0 (34 %; start of the kernel, the dependent reads of
+// length, table and keys, and the join are 10 of them), 131072 keys 91 (90 %), 262144 169 (98 %); B32 4096 keys 88 (94 %); at D64 131072
+// keys 55 (74 %), at D256 165 (98 %); 4 tokens of H64/8 against 131072 keys 120 (69 %).
 #include "sm100_ptx.cuh"
 #include "fa2_launch.h"
 #include "fa2_paged_params.h"
@@ -724,7 +733,7 @@ __device__ __forceinline__ void join_parts(const PagedParams& p, int c, int firs
 // mass[page][kv head][row] += sum over the query rows of exp2(score - maximum) / sum, four keys a thread; the sum is in the order of
 // the rows, and the addition is atomic because sequences may share a page. The rows' maxima and sums are those of the unit where
 // one CTA has it, else they come from the parts.
-__device__ __forceinline__ void add_weights(const PagedParams& p, int unit, int block, int blocks, int d, int unit_rows, float2* s_stats) {
+__device__ __forceinline__ void add_weights(const PagedParams& p, int grid, int unit, int block, int blocks, int d, int unit_rows, float2* s_stats) {
   const int b = unit / p.heads_k, hk = unit - b * p.heads_k;
   const int length = cut_length(p.seqlens[b], min(static_cast<int64_t>(p.most_keys), p.table.capacity()));
   const int lo = p.window < 0 ? 0 : max(0, length - p.seqlen_q - p.window);
@@ -736,7 +745,7 @@ __device__ __forceinline__ void add_weights(const PagedParams& p, int unit, int 
     const int rt = r / unit_rows, in = r - rt * unit_rows;
     const int2 parts = p.units[static_cast<int64_t>(unit) * p.row_tiles + rt];
     float2 stat;
-    if (parts.y == 0) {
+    if (parts.y <= 0 || parts.x < 0 || parts.y > grid - parts.x) {  // whole (or, of lengths that changed meanwhile, nothing that is known)
       stat = __ldcg(p.stats + static_cast<int64_t>(unit) * p.rows + r);
     } else {
       float top = -INFINITY, total = 0.f;
@@ -786,7 +795,7 @@ __global__ void __launch_bounds__(kTailThreads) paged_tail_kernel(const __grid_c
     join_parts<BF16>(p, i % grid, i / grid * 8, d, unit_rows);
   } else {
     const int unit = (i - joins) / blocks;
-    add_weights(p, unit, i - joins - unit * blocks, blocks, d, unit_rows, s_stats);
+    add_weights(p, grid, unit, i - joins - unit * blocks, blocks, d, unit_rows, s_stats);
   }
 }
 

@@ -164,6 +164,7 @@ BAD_CACHES = [(dict(size=8), -1, "size"), (dict(dtype=7), -2, "float16"), (dict(
               (dict(num_pages=0), -1, "positive"), (dict(page_size=-1), -1, "positive"), (dict(max_pages=0), -1, "positive"),
               (dict(batch=70000), -1, "65535"), (dict(heads_k=0), -1, "65535"), (dict(k=0), -1, "non-null"), (dict(block_table=0), -1, "non-null"),
               (dict(k=(1 << 20) + 8), -1, "aligned"), (dict(v_stride=(2048, 100, 64)), -1, "multiples of 8"),
+              (dict(block_table=(1 << 20) + 2), -1, "4-byte"), (dict(seqlens_k=(1 << 20) + 1), -1, "4-byte"), (dict(attn_mass=(1 << 20) + 3), -1, "4-byte"),
               (dict(k_stride=(2048, -128, 64)), -1, "negative"), (dict(reserved=1), -1, "reserved")]
 
 
@@ -196,7 +197,7 @@ def test_bad_turns_are_refused(built_libs, change, code, word):
 
 @pytest.mark.parametrize("change,code,word", [
     (dict(turn=dict(heads_k=4)), -1, "cache's heads"), (dict(turn=dict(head_dim=72)), -1, "cache's heads"), (dict(turn=dict(dtype=0)), -2, "dtype"),
-    (dict(turn=dict(k=0)), -1, "k is null"), (dict(turn=dict(batch=3)), -1, "batch"), (dict(cu_seqlens=1 << 20), -1, "cu_seqlens"),
+    (dict(turn=dict(k=0)), -1, "k is null"), (dict(turn=dict(batch=3)), -1, "batch"), (dict(cu_seqlens=1 << 20), -1, "cu_seqlens"), (dict(seqlens_new=(1 << 20) + 2), -1, "4-byte"),
     (dict(v=0), -1, "v must"), (dict(v=(1 << 20) + 1), -1, "v must"), (dict(size=8), -1, "size")], ids=str)
 def test_bad_appends_are_refused(built_libs, change, code, word):
     from flash_attn2_b200 import _cabi
@@ -212,14 +213,14 @@ def test_bad_appends_are_refused(built_libs, change, code, word):
 @pytest.mark.parametrize("change,word", [
     (dict(size=8), "size"), (dict(heads=3), "multiple"), (dict(heads=0), "multiple"), (dict(seqlen_q=-1), "seqlen_q"), (dict(seqlen_q=65), "128 query rows"),
     (dict(softmax_scale=float("nan")), "softmax_scale"), (dict(softcap=-1.0), "softcap"), (dict(softcap=float("inf")), "softcap"),
-    (dict(max_seqlen_k=-1), "max_seqlen_k"), (dict(q=0), "non-null"), (dict(out=0), "non-null"), (dict(lse=0), "non-null"),
+    (dict(max_seqlen_k=-1), "max_seqlen_k"), (dict(q=0), "non-null"), (dict(out=0), "non-null"), (dict(lse=0), "non-null"), (dict(lse=(1 << 20) + 2), "4-byte"),
     (dict(q=(1 << 20) + 2), "aligned"), (dict(o_stride=(256, 256, 60)), "multiples of 8")], ids=str)
 def test_bad_forwards_are_refused(built_libs, change, word):
     _refused("fa2_paged_fwd", _fwd(**change), -1, word, None, 0, None)
 
 
 @pytest.mark.parametrize("change,word", [
-    (dict(size=8), "size"), (dict(budget=0), "budget"), (dict(recent=-1), "recent"), (dict(recent=5), "recent"), (dict(dst_block_table=0), "dst_block_table"),
+    (dict(size=8), "size"), (dict(budget=0), "budget"), (dict(budget=2 ** 31 - 1), "budget"), (dict(kept=(1 << 20) + 1), "4-byte"), (dict(recent=-1), "recent"), (dict(recent=5), "recent"), (dict(dst_block_table=0), "dst_block_table"),
     (dict(dst_max_pages=0), "dst_block_table"), (dict(kept=0), "kept"), (dict(seqlens_out=0), "seqlens_out"), (dict(reserved=1), "reserved")], ids=str)
 def test_bad_evictions_are_refused(built_libs, change, word):
     from flash_attn2_b200 import _cabi

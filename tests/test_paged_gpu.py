@@ -2,6 +2,8 @@
 end inside tiles, every head-dim bucket, rows without keys, what lies in masked places, accumulated weights, graphs, streams, far offsets."""
 import ctypes as C
 import math
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -85,6 +87,95 @@ def test_attention(case, dtype):
     assert fa2.cabi_ops.device_status() == 0
 
 
+@pytest.mark.parametrize("page", [16, 24, 9])
+@pytest.mark.parametrize("d", [64, 104, 128, 192, 256])
+@pytest.mark.parametrize("h,hk,sq", [(5, 1, 1), (12, 1, 1), (16, 2, 3), (18, 2, 5)])
+def test_rows_dims_and_pages(page, d, h, hk, sq):
+    """Units of 8, 16 and 32 rows and of more (5, 12, 24, 45 rows), every head-dim bucket, whole and broken tiles."""
+    import flash_attn2_b200 as fa2
+
+    lengths = [700, 65, 2, 0, 1300]
+    k, v, table = make_cache(14, lengths, hk, d, page, torch.bfloat16)
+    q = torch.randn(5, sq, h, d, generator=torch.Generator().manual_seed(15)).bfloat16().cuda()
+    want = attend(q, k, v, table, lengths, window=600)
+    mass = torch.zeros(k.shape[0], hk, page, device="cuda")
+    out, lse = fa2.paged_fwd(q, k, v, table, _table(lengths), attn_mass=mass, window_size_left=600)
+    assert fa2.cabi_ops.device_status() == 0
+    _close(out, lse, want, torch.bfloat16, v, 700)
+    for b, n in enumerate(lengths):
+        got = mass[table[b].long().clamp(min=0)].transpose(1, 2).flatten(0, 1)[:n].T.cpu().double()
+        torch.testing.assert_close(got, want[2][b], rtol=2 ** -23, atol=2 * want[3] * sq * (h // hk))
+
+
+def test_scores_that_keep_growing():
+    """Keys in the order of their scores, over a range of 2^150: the running maximum moves many times, and early weights vanish."""
+    import flash_attn2_b200 as fa2
+
+    n, d = 2000, 64
+    k, v, table = make_cache(16, [n], 1, d, 16, torch.float16)
+    q = torch.zeros(1, 2, 4, d, dtype=torch.float16, device="cuda")
+    q[..., 0] = 8.0
+    ramp = torch.linspace(-52, 52, n).half()
+    for order in (ramp, ramp.flip(0)):
+        t = torch.arange(n)
+        k[table[0].long().cpu()[t // 16], t % 16, 0, 0] = order.cuda()
+        want = attend(q, k, v, table, [n])
+        out, lse = fa2.paged_fwd(q, k, v, table, _table([n]))
+        _close(out, lse, want, torch.float16, v, n)
+
+
+def test_heads_that_share_their_memory():
+    """A cache whose heads are one, expanded."""
+    import flash_attn2_b200 as fa2
+
+    k, v, table = make_cache(17, [300, 40], 1, 128, 16, torch.bfloat16)
+    q = torch.randn(2, 1, 8, 128, generator=torch.Generator().manual_seed(5)).bfloat16().cuda()
+    want = fa2.paged_fwd(q, k, v, table, _table([300, 40]))
+    got = fa2.paged_fwd(q, k.expand(-1, -1, 4, -1), v.expand(-1, -1, 4, -1), table.expand(2, -1), _table([300, 40]))
+    # the same products in units of other rows: the parts are cut elsewhere
+    torch.testing.assert_close(got[0], want[0], rtol=2 ** -7, atol=1e-4)
+    torch.testing.assert_close(got[1], want[1], rtol=0, atol=1e-5)
+
+
+def test_inference_mode_and_parameters():
+    import flash_attn2_b200 as fa2
+
+    k, v, table = make_cache(18, [30], 2, 64, 16, torch.bfloat16)
+    pos, freq = torch.full((1, 1, 1), 30, device="cuda"), torch.nn.Parameter(torch.rand(32, device="cuda"), requires_grad=False)
+    with torch.inference_mode():
+        x = torch.randn(1, 1, 2, 64, device="cuda").bfloat16()
+        own = k.clone()
+        q = fa2.paged_append(x, x, x, own, v.clone(), table, _table([30]), pos, freq, (32,))
+        assert torch.equal(q, fa2.rotary_axes_func(x, None, pos, freq, (32,))[0])
+        assert torch.equal(own[table[0, 1].long(), 14], q[0, 0])
+        fa2.paged_fwd(q, own, v, table, _table([30]))
+
+
+CAPTURE = r"""
+import sys
+sys.path[:0] = ["kernels-community-rs_b200"]
+import torch
+import flash_attn2_b200 as fa2
+k = torch.randn(8, 16, 2, 192, device="cuda", dtype=torch.float16)
+v, table, n = torch.randn_like(k), torch.arange(8, device="cuda", dtype=torch.int32).view(1, 8), torch.tensor([100], device="cuda", dtype=torch.int32)
+q, mass = torch.randn(1, 1, 4, 192, device="cuda", dtype=torch.float16), torch.zeros(8, 2, 16, device="cuda")
+x = torch.randn(1, 1, 2, 64, device="cuda", dtype=torch.float16)
+fa2.rotary_axes_func(x, None, torch.ones(1, 1, 1, device="cuda", dtype=torch.int32), torch.rand(32, device="cuda"), (32,))  # some call
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out, lse = fa2.paged_fwd(q, k, v, table, n, attn_mass=mass)
+graph.replay()
+torch.cuda.synchronize()
+assert torch.equal(out, fa2.paged_fwd(q, k, v, table, n)[0])
+print("done")
+"""
+
+
+def test_a_kernel_whose_first_call_is_captured():
+    run = subprocess.run([sys.executable, "-c", CAPTURE], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "done" in run.stdout, run.stdout + run.stderr[-2000:]
+
+
 def test_masked_places_may_hold_anything():
     """Infinities and NaN where some rows of a call see a key and others do not: only the rows that see it get them."""
     import flash_attn2_b200 as fa2
@@ -143,6 +234,11 @@ def test_views_of_q_and_out():
     for out in buffers:
         got = fa2.paged_fwd(q, k, v, table, _table(lengths), out=out)
         assert got[0] is out and torch.equal(out, want) and torch.equal(got[1], lse)
+    wide_out = torch.full((2, 4, h + 2, d + 8), 9.0).bfloat16().cuda()      # nothing is written around the output
+    fa2.paged_fwd(q, k, v, table, _table(lengths), out=wide_out[:, 1:3, 1:-1, :d])
+    assert torch.equal(wide_out[:, 1:3, 1:-1, :d], want)
+    wide_out[:, 1:3, 1:-1, :d] = 9.0
+    assert (wide_out == 9.0).all()
     same = q.clone()
     assert torch.equal(fa2.paged_fwd(same, k, v, table, _table(lengths), out=same)[0], want)
 
@@ -444,11 +540,30 @@ def _evict(fa2, lengths, budget, recent, hk, d, page, kind):
         assert torch.equal(now.cpu().view(word), w.view(word))
 
 
-def test_evict_from_more_than_shared_memory_holds():
+@pytest.mark.parametrize("lengths", [[60000, 49153, 100], [12000], [30000, 16385, 7], [140001]], ids=str)
+def test_evict_of_long_sequences(lengths):
+    """Clusters of 2, 4 and 8 CTAs, and more keys than their registers hold."""
     import flash_attn2_b200 as fa2
 
     for kind in ("heavy", "ties"):
-        _evict(fa2, [60000, 49153, 100], 20000, 300, 1, 8, 128, kind)
+        _evict(fa2, lengths, max(lengths) // 3, 300, 1, 8, 128 if kind == "ties" else 50, kind)
+
+
+def test_evict_of_many_long_sequences():
+    """More units than SMs: a CTA each, and more keys than its registers hold. (All rows go to one page: only the choice is looked at.)"""
+    import flash_attn2_b200 as fa2
+
+    b, n, page, budget = 150, 20000, 16, 5000
+    k = torch.zeros(n // page + 1, page, 1, 8, dtype=torch.float16, device="cuda")
+    mass = torch.randn(k.shape[0], 1, page, device="cuda").abs().round(decimals=2)
+    table = torch.arange(n // page, dtype=torch.int32, device="cuda").expand(b, -1)
+    lengths = torch.arange(n - b, n, device="cuda", dtype=torch.int32)
+    want = [mass[:-1].flatten()[: m - 10].sort(descending=True, stable=True).indices[: budget - 10].sort().values for m in lengths.tolist()]
+    got, kept = fa2.paged_evict(k, k.clone(), mass.clone(), table, lengths, torch.full((b, budget // page + 1), n // page, dtype=torch.int32, device="cuda"),
+                                budget, recent=10)
+    assert fa2.cabi_ops.device_status() == 0 and (got == budget).all()
+    for i, w in enumerate(want):
+        assert torch.equal(kept[i, 0, : budget - 10].long(), w) and kept[i, 0, -1] == lengths[i] - 1
 
 
 def test_evict_with_pages_that_cannot_be():
