@@ -8,8 +8,7 @@
 // Two kernels:
 //
 //   * The choice, a cluster of 1 to 8 CTAs per (sequence, kv head), so that few of them use more of the GPU. The weights become
-//     32-bit keys in the order of the numbers, 16 of them in each thread's registers; what does not fit is read again in every
-//     pass. A radix search from the top (11, 11 and 10 bits, a histogram each, the CTAs' added up over distributed shared memory)
+//     32-bit keys in the order of the numbers, in shared memory where they fit; else they are read again in every pass. A radix search from the top (11, 11 and 10 bits, a histogram each, the CTAs' added up over distributed shared memory)
 //     finds the key of the last one to be kept and how many of the keys equal to it are; one pass in the order of the tokens
 //     then writes the list of what is kept. It is bound by the latency of its steps: B2 Hk8 from 4096 tokens 12 us with one CTA each.
 //   * The move, all SMs: a row's 16-byte pieces by neighbouring threads, one of K and one of V in flight in each of 2048 threads per
@@ -28,8 +27,8 @@ namespace {
 
 constexpr int kSelectThreads = 1024;
 constexpr int kBins = 2048;
-constexpr int kRounds = 4;                            // groups of four neighbouring keys that a thread holds
-constexpr int kRoundKeys = 4 * kSelectThreads;
+constexpr int kRoundKeys = 4 * kSelectThreads;        // four neighbouring keys a thread
+constexpr int kHeld = 4 * kRoundKeys;                 // keys that shared memory holds
 
 // Larger numbers have larger keys; both zeroes are one, and NaN is above all.
 __device__ __forceinline__ uint32_t order_key(float f) {
@@ -39,43 +38,27 @@ __device__ __forceinline__ uint32_t order_key(float f) {
   return u >> 31 ? ~u : u | 0x80000000u;
 }
 
-// x[i] becomes the sum over the threads before this one, all[i] the sum over all.
-// The last N - n of them are left out: they are zero.
-template <int N>
-__device__ __forceinline__ void block_scan(int (&x)[N], int (&all)[N], int n, int (*s_warp)[32]) {
+// Sum over the threads before this one, and over all.
+__device__ __forceinline__ int block_scan(int x, int* s_warp, int& all) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int y[N];
+  int y = x;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    if (i >= n) break;
-    y[i] = x[i];
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int z = __shfl_up_sync(0xffffffffu, y[i], d);
-      if (lane >= d) y[i] += z;
-    }
+  for (int d = 1; d < 32; d <<= 1) {
+    const int z = __shfl_up_sync(0xffffffffu, y, d);
+    if (lane >= d) y += z;
   }
   __syncthreads();
-  if (lane == 31) {
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (i < n) s_warp[i][warp] = y[i];
-  }
+  if (lane == 31) s_warp[warp] = y;
   __syncthreads();
+  int w = s_warp[lane];
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    all[i] = 0;
-    if (i >= n) continue;
-    int w = s_warp[i][lane];
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int z = __shfl_up_sync(0xffffffffu, w, d);
-      if (lane >= d) w += z;
-    }
-    all[i] = __shfl_sync(0xffffffffu, w, 31);
-    const int before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
-    x[i] = y[i] - x[i] + (warp > 0 ? before : 0);
+  for (int d = 1; d < 32; d <<= 1) {
+    const int z = __shfl_up_sync(0xffffffffu, w, d);
+    if (lane >= d) w += z;
   }
+  all = __shfl_sync(0xffffffffu, w, 31);
+  const int before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
+  return y - x + (warp > 0 ? before : 0);
 }
 static_assert(kSelectThreads == 32 * 32, "the scan takes one warp sum a lane");
 
@@ -87,10 +70,18 @@ __device__ __forceinline__ int4 peer_words(const int* word, uint32_t rank) {
   return v;
 }
 
+__device__ __forceinline__ int peer_word(const int* word, uint32_t rank) {
+  int v;
+  asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(peer_smem(smem_u32(word), rank)) : "memory");
+  return v;
+}
+
 template <int CTAS>
 __global__ void __launch_bounds__(kSelectThreads, 1) evict_select_kernel(const __grid_constant__ EvictParams p) {
   __shared__ __align__(16) int s_bin[3][kBins];   // one for each pass: the other CTAs may still read the one before
-  __shared__ int s_warp[kRounds][32];
+  extern __shared__ __align__(16) uint4 s_key[];
+  __shared__ int s_eight[CTAS > 1 ? 3 : 1][kBins / 8];
+  __shared__ int s_warp[32];
   __shared__ __align__(16) int s_count[4];       // keys above and equal to the last one's
   __shared__ int s_found, s_above;
   const int tid = threadIdx.x;
@@ -150,30 +141,19 @@ __global__ void __launch_bounds__(kSelectThreads, 1) evict_select_kernel(const _
         }
     }
   };
-  const bool held = slice <= kRounds * kRoundKeys;
-  uint32_t key[kRounds][4];
+  const bool held = slice <= kHeld;
   if (held) {
-#pragma unroll
-    for (int r = 0; r < kRounds; ++r) {
-      const int i = begin + r * kRoundKeys + 4 * tid;
-      if (i < end) read(i, key[r]);
+    for (int i = begin + 4 * tid; i < end; i += kRoundKeys) {
+      uint32_t k[4];
+      read(i, k);
+      s_key[(i - begin) / 4] = make_uint4(k[0], k[1], k[2], k[3]);
     }
   }
-  // Calls f(first token, its four keys) for this thread's groups of four.
-  auto visit = [&](auto&& f) {
-    if (held) {
-#pragma unroll
-      for (int r = 0; r < kRounds; ++r) {
-        const int i = begin + r * kRoundKeys + 4 * tid;
-        if (i < end) f(i, key[r]);
-      }
-    } else {
-      for (int i = begin + 4 * tid; i < end; i += kRoundKeys) {
-        uint32_t k[4];
-        read(i, k);
-        f(i, k);
-      }
-    }
+  // Four keys of this thread's own.
+  auto keys = [&](int i, uint32_t (&k)[4]) {
+    if (!held) return read(i, k);
+    const uint4 w = s_key[(i - begin) / 4];
+    k[0] = w.x, k[1] = w.y, k[2] = w.z, k[3] = w.w;
   };
 
   // ---- the key of the last one to be kept: `prefix` are its bits so far, `above` counts the larger keys
@@ -184,26 +164,30 @@ __global__ void __launch_bounds__(kSelectThreads, 1) evict_select_kernel(const _
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
     int* bin = s_bin[pass];
-    visit([&](int i, const uint32_t (&k)[4]) {
+#pragma unroll 1
+    for (int i = begin + 4 * tid; i < end; i += kRoundKeys) {
+      uint32_t k[4];
+      keys(i, k);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (i + e < end && (pass == 0 || k[e] >> (shift + bits) == prefix)) atomicAdd(&bin[(k[e] >> shift) & ((1u << bits) - 1)], 1);
-    });
-    meet();
-    // Threads 0 to 255 have eight bins each, from the top.
-    int sum[8] = {}, mine = 0;
+    }
+    // Threads 0 to 255 have eight bins each, from the top. The CTAs exchange the sums of eight first, and of the eight in question the bins.
+    const int* eight = bin + kBins - 8 - 8 * tid;
+    int mine = 0;
+    __syncthreads();
     if (tid < kBins / 8) {
+      const int4 v = *reinterpret_cast<const int4*>(eight), w = *reinterpret_cast<const int4*>(eight + 4);
+      mine = v.x + v.y + v.z + v.w + w.x + w.y + w.z + w.w;
+    }
+    if constexpr (CTAS > 1) {
+      if (tid < kBins / 8) s_eight[pass][tid] = mine;
+      meet();
+      if (tid < kBins / 8) {
+        mine = 0;
 #pragma unroll
-      for (int r = 0; r < CTAS; ++r) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int* from = bin + kBins - 8 * tid - 4 - 4 * h;
-          const int4 v = CTAS > 1 ? peer_words(from, r) : *reinterpret_cast<const int4*>(from);
-          sum[4 * h] += v.w, sum[4 * h + 1] += v.z, sum[4 * h + 2] += v.y, sum[4 * h + 3] += v.x;
-        }
+        for (int r = 0; r < CTAS; ++r) mine += peer_word(&s_eight[pass][tid], r);
       }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) mine += sum[e];
     }
     int upto = mine;  // keys in this thread's bins and above, of those that this pass looks at
     if (tid < kBins / 8) {
@@ -212,22 +196,33 @@ __global__ void __launch_bounds__(kSelectThreads, 1) evict_select_kernel(const _
         const int z = __shfl_up_sync(0xffffffffu, upto, d);
         if ((tid & 31) >= d) upto += z;
       }
-      if ((tid & 31) == 31) s_warp[0][tid >> 5] = upto;
+      if ((tid & 31) == 31) s_warp[tid >> 5] = upto;
     }
     __syncthreads();
     if (tid < kBins / 8) {
       upto += above - mine;
-      for (int w = 0; w < tid >> 5; ++w) upto += s_warp[0][w];
-      if (upto < wanted && upto + mine >= wanted) {
-        int e = 0;
-        while (upto + sum[0] < wanted) {  // shifts, so that the sums stay in registers
-          upto += sum[0];
-          ++e;
 #pragma unroll
-          for (int k = 0; k < 7; ++k) sum[k] = sum[k + 1];
+      for (int w = 0; w < kBins / 256; ++w)
+        if (w < tid >> 5) upto += s_warp[w];
+      if (upto < wanted && upto + mine >= wanted) {
+#pragma unroll
+        for (int h = 1; h >= 0; --h) {
+          int4 v = make_int4(0, 0, 0, 0);
+#pragma unroll
+          for (int r = 0; r < CTAS; ++r) {
+            const int4 x = CTAS > 1 ? peer_words(eight + 4 * h, r) : *reinterpret_cast<const int4*>(eight + 4 * h);
+            v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+          }
+          const int count[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int e = 3; e >= 0; --e) {
+            if (upto < wanted && upto + count[e] >= wanted) {
+              s_found = kBins - 8 - 8 * tid + 4 * h + e;
+              s_above = upto;
+            }
+            upto += count[e];
+          }
         }
-        s_found = kBins - 1 - 8 * tid - e;
-        s_above = upto;
       }
     }
     __syncthreads();
@@ -242,14 +237,17 @@ __global__ void __launch_bounds__(kSelectThreads, 1) evict_select_kernel(const _
   int done_above = 0, done_ties = 0;
   if constexpr (CTAS > 1) {
     int larger = 0, equal = 0;
-    visit([&](int i, const uint32_t (&k)[4]) {
+#pragma unroll 1
+    for (int i = begin + 4 * tid; i < end; i += kRoundKeys) {
+      uint32_t k[4];
+      keys(i, k);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (i + e < end) {
           larger += k[e] > prefix;
           equal += k[e] == prefix;
         }
-    });
+    }
     larger = __reduce_add_sync(0xffffffffu, larger);
     equal = __reduce_add_sync(0xffffffffu, equal);
     if ((tid & 31) == 0) {
@@ -268,33 +266,30 @@ __global__ void __launch_bounds__(kSelectThreads, 1) evict_select_kernel(const _
     __syncwarp();
     cluster_arrive();  // no CTA ends while another one reads its shared memory
   }
-  for (int i0 = begin; i0 < end; i0 += kRounds * kRoundKeys) {
-    int count[kRounds], all[kRounds];  // larger ones in the lower half, equal ones in the upper half: at most 4096 each
-#pragma unroll
-    for (int r = 0; r < kRounds; ++r) {
-      const int i = i0 + r * kRoundKeys + 4 * tid;
-      count[r] = 0;
-      if (!held && i < end) read(i, key[r]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (i + e < end) count[r] += (key[r][e] > prefix ? 1 : 0) + (key[r][e] == prefix ? 1 << 16 : 0);
-    }
-    block_scan(count, all, min(kRounds, (end - i0 + kRoundKeys - 1) / kRoundKeys), s_warp);
-#pragma unroll
-    for (int r = 0; r < kRounds; ++r) {
-      const int i = i0 + r * kRoundKeys + 4 * tid;
-      int at_above = done_above + (count[r] & 0xffff), at_ties = done_ties + (count[r] >> 16);
+#pragma unroll 1
+  for (int i0 = begin; i0 < end && (done_above < above || done_ties < ties); i0 += kRoundKeys) {
+    const int i = i0 + 4 * tid;
+    uint32_t k[4];
+    int count = 0;  // larger ones in the lower half, equal ones in the upper half: at most 4096 each
+    if (i < end) {
+      keys(i, k);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (i + e < end) {
-          const bool larger = key[r][e] > prefix, tie = key[r][e] == prefix;
-          if (larger || (tie && at_ties < ties)) kept[at_above + min(at_ties, ties)] = i + e;
-          at_above += larger;
-          at_ties += tie;
-        }
-      done_above += all[r] & 0xffff;
-      done_ties += all[r] >> 16;
+        if (i + e < end) count += (k[e] > prefix ? 1 : 0) + (k[e] == prefix ? 1 << 16 : 0);
     }
+    int all;
+    const int before = block_scan(count, s_warp, all);
+    int at_above = done_above + (before & 0xffff), at_ties = done_ties + (before >> 16);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (i + e < end) {
+        const bool larger = k[e] > prefix, tie = k[e] == prefix;
+        if (larger || (tie && at_ties < ties)) kept[at_above + min(at_ties, ties)] = i + e;
+        at_above += larger;
+        at_ties += tie;
+      }
+    done_above += all & 0xffff;
+    done_ties += all >> 16;
   }
   if constexpr (CTAS > 1) {
     __syncwarp();
@@ -341,7 +336,17 @@ namespace {
 
 template <int CTAS>
 cudaError_t launch_select(const EvictParams& p, cudaStream_t stream) {
-  return launch_clusters(CTAS, evict_select_kernel<CTAS>, dim3(static_cast<unsigned>(p.batch * p.heads_k) * CTAS), kSelectThreads, 0, stream, p);
+  static bool configured[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && !configured[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(evict_select_kernel<CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeld * 4);
+    if (e != cudaSuccess) return e;
+    configured[dev] = true;
+  }
+  const int64_t slice = (p.from.capacity() / CTAS + 8) / 4 * 4;  // the most that a CTA can have
+  return launch_clusters(CTAS, evict_select_kernel<CTAS>, dim3(static_cast<unsigned>(p.batch * p.heads_k) * CTAS), kSelectThreads,
+                         static_cast<size_t>(std::min<int64_t>(slice, kHeld)) * 4, stream, p);
 }
 
 }  // namespace
