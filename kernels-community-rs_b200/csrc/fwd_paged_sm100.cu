@@ -25,8 +25,8 @@
 //   * Keys that no row sees are not read or count as zero, whatever lies there. Where some rows see a key and others do not, P's
 //     zero meets its value, and a value that is not finite would make a NaN of it: such values take a path of their own.
 //
-// Measured (us a call, share of the measured copy rate): B1 H32/8 D128 8192 keys 15.0 (34 %; start of the kernel, the dependent reads of
-// length, table and keys, and the join are 10 of them), 131072 keys 91 (90 %), 262144 169 (98 %); B32 4096 keys 88 (94 %); at D64 131072
+// Measured (us a call, share of the measured copy rate): B1 H32/8 D128 8192 keys 13.9 (37 %; start of the kernel, the dependent reads of
+// length, table and keys, and the join are 8 of them), 131072 keys 91 (90 %), 262144 169 (98 %); B32 4096 keys 88 (94 %); at D64 131072
 // keys 55 (74 %), at D256 165 (98 %); 4 tokens of H64/8 against 131072 keys 120 (69 %).
 #include "sm100_ptx.cuh"
 #include "fa2_launch.h"
@@ -675,58 +675,65 @@ __global__ void __launch_bounds__((Cfg<A, NT, TEAM>::kThreads), 1) fwd_paged_ker
 // ---- what is left when the parts are there: the units that several CTAs share, and the weights. A kernel of its own, which starts
 // early and waits beside the attention. (With flags in memory, by which the last CTA of a unit knew itself, a call ended with two fences
 // and two round trips to memory: B1 H32/8 Sk 8192 D128 17.3 us in place of 14.9.)
-constexpr int kTailThreads = 128;  // its registers fit beside those of the attention
+constexpr int kTailThreads = 128;
 
 // Slot 2 c holds the part of a segment that began before CTA c's share, 2 c + 1 that of one that began in it: the first part.
 __device__ __forceinline__ const float* part_of(const PagedParams& p, int c_first, int i, int64_t slot) {
   return p.partials + (2 * static_cast<int64_t>(c_first + i) + (i == 0 ? 1 : 0)) * slot;
 }
 
-// Adds up the parts of 8 rows (from `first_row` on) of the unit that begins in share c, in the order of the keys.
+// A row's maximum, sum and four columns, and the same with another part added.
+struct RowPart {
+  float top, total;
+  float4 acc;
+};
+__device__ __forceinline__ void add_part(RowPart& a, float top, float total, const float4& v) {
+  const float above = fmaxf(a.top, top), f = part_scale(a.top, above), g = part_scale(top, above);
+  a.top = above;
+  a.total = f * a.total + g * total;
+  a.acc.x = f * a.acc.x + g * v.x;
+  a.acc.y = f * a.acc.y + g * v.y;
+  a.acc.z = f * a.acc.z + g * v.z;
+  a.acc.w = f * a.acc.w + g * v.w;
+}
+
+// Adds up the parts of a row of the unit that begins in share c, in the order of the keys: a block has a row, a thread four columns
+// of some neighbouring parts. (A single unit of 8192 keys at D256 comes in 128 parts.)
 template <bool BF16>
-__device__ __forceinline__ void join_parts(const PagedParams& p, int c, int first_row, int d, int unit_rows) {
+__device__ __forceinline__ void join_parts(const PagedParams& p, int c, int r, int d, int unit_rows, RowPart* s_part) {
   const int4 unit = p.shared[c];
-  const int n_parts = unit.x;
-  if (n_parts == 0) return;
-  const int row0 = unit.w * unit_rows + first_row, rows = min(8, min(unit_rows - first_row, p.rows - row0));
+  const int n_parts = unit.x, row = unit.w * unit_rows + r;
+  if (n_parts == 0 || row >= p.rows) return;
   const int64_t slot = static_cast<int64_t>(unit_rows) * (d + 2);
-  for (int i = threadIdx.x; i < rows * (d / 4); i += kTailThreads) {
-    const int r = first_row + i / (d / 4), col = i % (d / 4) * 4;
-    float top = -INFINITY, total = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    constexpr int kBatch = 10;  // parts whose loads are in flight together
-    for (int c0 = 0; c0 < n_parts; c0 += kBatch) {
+  const int columns = d / 4, groups = kTailThreads / columns, group = threadIdx.x / columns, col = (threadIdx.x - group * columns) * 4;
+  const int per = (n_parts + groups - 1) / groups, end = min(n_parts, (group + 1) * per);
+  RowPart sum{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+  if (group < groups) {
+    constexpr int kBatch = 8;  // parts whose loads are in flight together
+    for (int c0 = group * per; c0 < end; c0 += kBatch) {
       float4 v[kBatch];
       float pm[kBatch], pl[kBatch];
 #pragma unroll
-      for (int e = 0; e < kBatch; ++e) {
-        pm[e] = -INFINITY;
-        if (c0 + e < n_parts) {
+      for (int e = 0; e < kBatch; ++e)
+        if (c0 + e < end) {
           const float* src = part_of(p, c, c0 + e, slot);
           v[e] = __ldcg(reinterpret_cast<const float4*>(src + r * d + col));
           pm[e] = __ldcg(src + unit_rows * d + r);
           pl[e] = __ldcg(src + unit_rows * d + unit_rows + r);
         }
-      }
-      float above = top;
-#pragma unroll
-      for (int e = 0; e < kBatch; ++e) above = fmaxf(above, pm[e]);
-      const float f = part_scale(top, above);
-      total *= f;
-      acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
-      top = above;
 #pragma unroll
       for (int e = 0; e < kBatch; ++e)
-        if (c0 + e < n_parts) {
-          const float g = part_scale(pm[e], top);
-          total += g * pl[e];
-          acc.x += g * v[e].x;
-          acc.y += g * v[e].y;
-          acc.z += g * v[e].z;
-          acc.w += g * v[e].w;
-        }
+        if (c0 + e < end) add_part(sum, pm[e], pl[e], v[e]);
     }
-    store_row<BF16>(p, unit.y, unit.z, unit.w * unit_rows + r, col, acc, top, total);
+    if (group > 0) s_part[threadIdx.x] = sum;
+  }
+  __syncthreads();
+  if (group == 0) {
+    for (int x = 1; x < groups && x * per < n_parts; ++x) {
+      const RowPart o = s_part[threadIdx.x + x * columns];
+      add_part(sum, o.top, o.total, o.acc);
+    }
+    store_row<BF16>(p, unit.y, unit.z, row, col, sum.acc, sum.top, sum.total);
   }
 }
 
@@ -784,18 +791,21 @@ __device__ __forceinline__ void add_weights(const PagedParams& p, int grid, int 
   }
 }
 
-// Blocks: `joins` for the shared units, 8 rows each, then `blocks` for the weights of each (sequence, kv head).
+// Blocks: `joins` for the rows of the shared units, then `blocks` for the weights of each (sequence, kv head).
 template <bool BF16>
 __global__ void __launch_bounds__(kTailThreads) paged_tail_kernel(const __grid_constant__ PagedParams p, int grid, int joins, int blocks, int d, int unit_rows) {
-  __shared__ float2 s_stats[kPagedMaxRows];
+  __shared__ union {
+    float2 stats[kPagedMaxRows];
+    RowPart part[kTailThreads];
+  } s;
   early_wait();
   early_trigger();
   const int i = blockIdx.x;
   if (i < joins) {
-    join_parts<BF16>(p, i % grid, i / grid * 8, d, unit_rows);
+    join_parts<BF16>(p, i % grid, i / grid, d, unit_rows, s.part);
   } else {
     const int unit = (i - joins) / blocks;
-    add_weights(p, grid, unit, i - joins - unit * blocks, blocks, d, unit_rows, s_stats);
+    add_weights(p, grid, unit, i - joins - unit * blocks, blocks, d, unit_rows, s.stats);
   }
 }
 
@@ -843,7 +853,7 @@ cudaError_t launch_fwd_paged(const PagedParams& p, int grid, int sm_count, bool 
   if (p.rows <= 0 || p.rows > kPagedMaxRows || p.head_dim <= 0 || p.head_dim > 256 || grid <= 0) return cudaErrorInvalidValue;
   const cudaError_t e = bf16 ? pick_dim<true>(p, grid, stream) : pick_dim<false>(p, grid, stream);
   if (e != cudaSuccess) return e;
-  const int d = (p.head_dim + 63) / 64 * 64, unit_rows = paged_unit_rows(p.rows), joins = grid * (unit_rows / 8);
+  const int d = (p.head_dim + 63) / 64 * 64, unit_rows = paged_unit_rows(p.rows), joins = grid * (p.rows < unit_rows ? p.rows : unit_rows);
   // Blocks for every key that there can be, but no more than fill the GPU a few times over: lengths are known on the device only.
   const int64_t units = static_cast<int64_t>(p.batch) * p.heads_k, keys = 4 * kTailThreads;
   const int64_t every = (static_cast<int64_t>(p.most_keys) + 3 + keys - 1) / keys, fill = (32 * static_cast<int64_t>(sm_count) + units - 1) / units;

@@ -10,9 +10,9 @@
 //   * The choice, a cluster of 1 to 8 CTAs per (sequence, kv head), so that few of them use more of the GPU. The weights become
 //     32-bit keys in the order of the numbers, in shared memory where they fit; else they are read again in every pass. A radix search from the top (11, 11 and 10 bits, a histogram each, the CTAs' added up over distributed shared memory)
 //     finds the key of the last one to be kept and how many of the keys equal to it are; one pass in the order of the tokens
-//     then writes the list of what is kept. It is bound by the latency of its steps: B2 Hk8 from 4096 tokens 12 us with one CTA each.
+//     then writes the list of what is kept. It is bound by the latency of its steps, a few thousand cycles.
 //   * The move, all SMs: a row's 16-byte pieces by neighbouring threads, one of K and one of V in flight in each of 2048 threads per
-//     SM. (Two or four rows a thread, and fewer threads, are slower: B16 Hk4 16384 -> 6000 87 and 92 us a call in place of 83.)
+//     SM. (Two or four rows a thread, and fewer threads, are slower: B16 Hk4 16384 -> 6000 87 and 92 us a call where one took 83.)
 //     Sources and destinations are different pages, so that the rows can move in any order and pages shared with another
 //     sequence stay as they are.
 #include <algorithm>
@@ -355,8 +355,8 @@ cudaError_t launch_paged_evict(const EvictParams& p, int sm_count, cudaStream_t 
   const int units = p.batch * p.heads_k;
   const int64_t most = p.from.capacity();
   // Clusters where there are SMs for them and more than 8192 keys for a CTA: their barriers and the exchange take longer than that many
-  // keys. us a call of B2 Hk8 from 4096 tokens with 1, 2, 4, 8 CTAs: 16.3, 19.2, 20.9, 39.8; of B16 Hk4 from 16384: 93.0, 92.9, 106.5,
-  // 164; of B1 Hk8 from 131072: 226, 183, 147, 123.
+  // keys. us a call of B2 Hk8 from 4096 tokens with 1 CTA 12.8, with 2 15.8; of B16 Hk4 from 16384 with 1 81.9, with 2 80.6; of B1 Hk8
+  // from 131072 with 1 226, with 8 104 (an earlier state: 226, 183, 147 and 123 with 1, 2, 4 and 8).
   const int64_t ctas = std::min<int64_t>((most + 8191) / 8192, sm_count / units);
   cudaError_t e = ctas >= 8 ? launch_select<8>(p, stream) : ctas >= 4 ? launch_select<4>(p, stream) : ctas >= 2 ? launch_select<2>(p, stream)
                                                                                                              : launch_select<1>(p, stream);
