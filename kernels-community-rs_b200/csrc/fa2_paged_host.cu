@@ -167,10 +167,11 @@ int plan_fwd(const fa2_paged_fwd_args* a, int sm_count, FwdPlan* f) {
   f->grid = static_cast<int>(std::min<int64_t>(sm_count, (most_tiles + fa2::kPagedMinShare - 1) / fa2::kPagedMinShare));
   f->list_bytes = round256(static_cast<int64_t>(f->grid) * 16);
   f->part_bytes = round256(2 * static_cast<int64_t>(f->grid) * fa2::paged_part_floats(c->head_dim, f->rows) * 4);
+  const int64_t units = static_cast<int64_t>(c->batch) * c->heads_k * f->row_tiles;
+  if (c->attn_mass != nullptr || fa2::paged_join_by_unit(units, f->grid, f->rows)) f->unit_bytes = round256(units * 8);
   if (c->attn_mass != nullptr) {
     const int64_t rows = static_cast<int64_t>(c->batch) * c->heads_k * f->rows;
     f->score_stride = (f->most_keys + 15) / 16 * 16;
-    f->unit_bytes = round256(static_cast<int64_t>(c->batch) * c->heads_k * f->row_tiles * 8);
     f->stat_bytes = round256(rows * 8);
     if (rows > (INT64_MAX >> 8) / f->score_stride) return fail(FA2_E_VALUE, "the scores of this call do not fit an address space");
     f->score_bytes = round256(rows * f->score_stride * 4);
@@ -317,8 +318,9 @@ int fa2_paged_fwd(const fa2_paged_fwd_args* args, void* workspace, int64_t works
   char* at = static_cast<char*>(workspace);
   p.shared = reinterpret_cast<int4*>(at);
   p.partials = reinterpret_cast<float*>(at += f.list_bytes);
+  at += f.part_bytes;
+  if (f.unit_bytes > 0) p.units = reinterpret_cast<int2*>(at);
   if (c->attn_mass != nullptr) {
-    p.units = reinterpret_cast<int2*>(at += f.part_bytes);
     p.stats = reinterpret_cast<float2*>(at += f.unit_bytes);
     p.scores = reinterpret_cast<float*>(at += f.stat_bytes);
     p.score_stride = f.score_stride;

@@ -27,7 +27,7 @@
 //
 // Measured (us a call, share of the measured copy rate): B1 H32/8 D128 8192 keys 13.9 (37 %; start of the kernel, the dependent reads of
 // length, table and keys, and the join are 8 of them), 131072 keys 91 (90 %), 262144 169 (98 %); B32 4096 keys 88 (94 %); at D64 131072
-// keys 55 (74 %), at D256 165 (98 %); 4 tokens of H64/8 against 131072 keys 120 (69 %).
+// keys 55 (74 %), at D256 165 (98 %); 4 tokens of H64/8 against 131072 keys 117 (71 %).
 #include "sm100_ptx.cuh"
 #include "fa2_launch.h"
 #include "fa2_paged_params.h"
@@ -697,11 +697,20 @@ __device__ __forceinline__ void add_part(RowPart& a, float top, float total, con
   a.acc.w = f * a.acc.w + g * v.w;
 }
 
-// Adds up the parts of a row of the unit that begins in share c, in the order of the keys: a block has a row, a thread four columns
-// of some neighbouring parts. (A single unit of 8192 keys at D256 comes in 128 parts.)
+// Adds up the parts of row r of a unit, in the order of the keys: a block has a row, a thread four columns of some neighbouring
+// parts. (A single unit of 8192 keys at D256 comes in 128 parts.) i: a unit (by_unit), or the CTA whose share the unit begins in.
 template <bool BF16>
-__device__ __forceinline__ void join_parts(const PagedParams& p, int c, int r, int d, int unit_rows, RowPart* s_part) {
-  const int4 unit = p.shared[c];
+__device__ __forceinline__ void join_parts(const PagedParams& p, int i, int r, bool by_unit, int d, int unit_rows, RowPart* s_part) {
+  int c = i;
+  int4 unit;  // parts, sequence, kv head, row tile
+  if (by_unit) {
+    const int2 parts = p.units[i];
+    const int b = i / (p.heads_k * p.row_tiles), rest = i - b * (p.heads_k * p.row_tiles), hk = rest / p.row_tiles;
+    c = parts.x;
+    unit = make_int4(parts.y, b, hk, rest - hk * p.row_tiles);
+  } else {
+    unit = p.shared[c];
+  }
   const int n_parts = unit.x, row = unit.w * unit_rows + r;
   if (n_parts == 0 || row >= p.rows) return;
   const int64_t slot = static_cast<int64_t>(unit_rows) * (d + 2);
@@ -791,9 +800,10 @@ __device__ __forceinline__ void add_weights(const PagedParams& p, int grid, int 
   }
 }
 
-// Blocks: `joins` for the rows of the shared units, then `blocks` for the weights of each (sequence, kv head).
+// Blocks: `joins` for the rows of the shared units, of which there are `listed` at most, then `blocks` for the weights of each
+// (sequence, kv head).
 template <bool BF16>
-__global__ void __launch_bounds__(kTailThreads) paged_tail_kernel(const __grid_constant__ PagedParams p, int grid, int joins, int blocks, int d, int unit_rows) {
+__global__ void __launch_bounds__(kTailThreads) paged_tail_kernel(const __grid_constant__ PagedParams p, int grid, int listed, int joins, int blocks, int d, int unit_rows) {
   __shared__ union {
     float2 stats[kPagedMaxRows];
     RowPart part[kTailThreads];
@@ -802,7 +812,7 @@ __global__ void __launch_bounds__(kTailThreads) paged_tail_kernel(const __grid_c
   early_trigger();
   const int i = blockIdx.x;
   if (i < joins) {
-    join_parts<BF16>(p, i % grid, i / grid, d, unit_rows, s.part);
+    join_parts<BF16>(p, i % listed, i / listed, listed != grid, d, unit_rows, s.part);
   } else {
     const int unit = (i - joins) / blocks;
     add_weights(p, grid, unit, i - joins - unit * blocks, blocks, d, unit_rows, s.stats);
@@ -853,14 +863,16 @@ cudaError_t launch_fwd_paged(const PagedParams& p, int grid, int sm_count, bool 
   if (p.rows <= 0 || p.rows > kPagedMaxRows || p.head_dim <= 0 || p.head_dim > 256 || grid <= 0) return cudaErrorInvalidValue;
   const cudaError_t e = bf16 ? pick_dim<true>(p, grid, stream) : pick_dim<false>(p, grid, stream);
   if (e != cudaSuccess) return e;
-  const int d = (p.head_dim + 63) / 64 * 64, unit_rows = paged_unit_rows(p.rows), joins = grid * (p.rows < unit_rows ? p.rows : unit_rows);
-  // Blocks for every key that there can be, but no more than fill the GPU a few times over: lengths are known on the device only.
   const int64_t units = static_cast<int64_t>(p.batch) * p.heads_k, keys = 4 * kTailThreads;
+  const int d = (p.head_dim + 63) / 64 * 64, unit_rows = paged_unit_rows(p.rows);
+  const int listed = paged_join_by_unit(units * p.row_tiles, grid, p.rows) ? static_cast<int>(units) * p.row_tiles : grid;
+  const int joins = listed * (p.rows < unit_rows ? p.rows : unit_rows);
+  // Blocks for every key that there can be, but no more than fill the GPU a few times over: lengths are known on the device only.
   const int64_t every = (static_cast<int64_t>(p.most_keys) + 3 + keys - 1) / keys, fill = (32 * static_cast<int64_t>(sm_count) + units - 1) / units;
   const int blocks = p.mass != nullptr ? static_cast<int>(every < fill ? every : fill) : 0;
   const dim3 all(static_cast<unsigned>(joins + units * blocks));
-  if (bf16) return launch_grid(true, paged_tail_kernel<true>, all, kTailThreads, 0, stream, p, grid, joins, blocks, d, unit_rows);
-  return launch_grid(true, paged_tail_kernel<false>, all, kTailThreads, 0, stream, p, grid, joins, blocks, d, unit_rows);
+  if (bf16) return launch_grid(true, paged_tail_kernel<true>, all, kTailThreads, 0, stream, p, grid, listed, joins, blocks, d, unit_rows);
+  return launch_grid(true, paged_tail_kernel<false>, all, kTailThreads, 0, stream, p, grid, listed, joins, blocks, d, unit_rows);
 }
 
 }  // namespace fa2
