@@ -8,9 +8,10 @@
 // Two kernels:
 //
 //   * The choice, a cluster of 1 to 8 CTAs per (sequence, kv head), so that few of them use more of the GPU. The weights become
-//     32-bit keys in the order of the numbers, in shared memory where they fit; else they are read again in every pass. A radix search from the top (11, 11 and 10 bits, a histogram each, the CTAs' added up over distributed shared memory)
-//     finds the key of the last one to be kept and how many of the keys equal to it are; one pass in the order of the tokens
-//     then writes the list of what is kept. It is bound by the latency of its steps, a few thousand cycles.
+//     32-bit keys in the order of the numbers, in shared memory where they fit; else they are read again in every pass. A radix
+//     search from the top (11, 11 and 10 bits, a histogram each, the CTAs' added up over distributed shared memory) finds the key
+//     of the last one to be kept and how many of the keys equal to it are; one pass in the order of the tokens then writes the
+//     list of what is kept. It is bound by the latency of its steps, a few thousand cycles.
 //   * The move, all SMs: a row's 16-byte pieces by neighbouring threads, one of K and one of V in flight in each of 2048 threads per
 //     SM. (Two or four rows a thread, and fewer threads, are slower: B16 Hk4 16384 -> 6000 87 and 92 us a call where one took 83.)
 //     Sources and destinations are different pages, so that the rows can move in any order and pages shared with another
