@@ -10,9 +10,10 @@
 //     of all (sequence, kv head, row tile, key tile); a share may begin and end inside a unit. A CTA leaves its part of a unit that it
 //     does not cover alone in the workspace, and a second kernel, which waits beside the first, adds the parts up (and the keys' weights).
 //   * Each warp walks key tiles of its own and keeps a queue of two or more of them in flight, 130 to 170 KB per SM: TMA boxes of 64
-//     columns where a tile lies in one page, else copies of 16 bytes by cp.async, of which an SM has only some 32 KB in flight. (One
-//     bulk copy for each row, for any page size, took 14 cycles a row: 18 B/clk per SM, where memory gives 29.) The queue goes on
-//     over the ends of units: the next unit's copies start before the warps' parts of the last one are added up.
+//     columns where a tile lies in one page, else copies of 16 bytes by cp.async, a row's neighbouring pieces by neighbouring lanes
+//     (131072 keys of 8 heads at D128 in pages of 100 96 us, in pages of 64 91). One bulk copy for each row, for any page size, took
+//     14 cycles a row: 18 B/clk per SM, where memory gives 29. The queue goes on over the ends of units: the next unit's copies
+//     start before the warps' parts of the last one are added up.
 //   * The products are transposed, S^T = K Q^T and O^T = V^T P^T, by mma.sync m16n8k16: the keys (the columns of V) are the 16, 8
 //     query rows the 8, so that 8 rows, one token's heads in most models, waste nothing. Which d a k index means is free as long as
 //     K and Q agree, and so is which column of V a row of O^T is: a lane reads 16 bytes of shared memory at a time, and the
