@@ -170,6 +170,9 @@ __global__ void __launch_bounds__((Cfg<A, NT, TEAM>::kThreads), 1) fwd_paged_ker
     s_before = 0;
     s_length = 0;
   }
+  // The warps' first waits read s_abort, and an elected lane arms barriers that other lanes have set up: nothing else orders these
+  // for short batches. It stands beside the end of the grid before.
+  __syncthreads();
   early_wait();
   early_trigger();
 

@@ -286,3 +286,28 @@ def test_cpu_tensors_and_wrong_types_are_refused(built_libs):
         fa.rotary_axes_func(None, None, pos, freq, (32,))
     with pytest.raises(TypeError):
         fa.paged_evict(cache, cache, mass, table, n, table, 4.0)
+
+
+# ---------------------------------------------------------------- what the kernels' source has to say
+def _kernels_with_barriers():
+    """(file, name, body from the barriers' set-up on) of each kernel that sets up mbarriers."""
+    import re
+
+    for path in sorted((ROOT / "kernels-community-rs_b200" / "csrc").glob("*.cu")):
+        for kernel in re.split(r"^(?=__global__ )", path.read_text(), flags=re.M)[1:]:
+            kernel = kernel[:kernel.index("\n}\n")]
+            if "mbar_init(" in kernel:
+                yield path.name, re.search(r"\b(\w+_kernel)\(", kernel)[1], kernel[kernel.rindex("mbar_fence_init()"):]
+
+
+def test_barriers_and_abort_words_are_seen_by_all_warps_before_their_first_wait():
+    """A block barrier that no condition guards (two spaces deep) stands between the set-up of a kernel's mbarriers and abort word and
+    the first wait. What a missing one does depends on the warps' timing, so that no run would show it."""
+    import re
+
+    found = list(_kernels_with_barriers())
+    assert {"fwd_paged_kernel", "fwd_kernel", "fwd_decode_kernel", "bwd_kernel"} <= {name for _, name, _ in found}
+    for path, name, body in found:
+        barrier = re.search(r"^  __syncthreads\(\);", body, flags=re.M)
+        assert barrier is not None, (path, name)
+        assert not re.search(r"(warp|mbar)_wait", body[:barrier.start()]), (path, name)
