@@ -704,7 +704,7 @@ __device__ __forceinline__ void add_part(RowPart& a, float top, float total, con
 // Adds up the parts of row r of a unit, in the order of the keys: a block has a row, a thread four columns of some neighbouring
 // parts. (A single unit of 8192 keys at D256 comes in 128 parts.) i: a unit (by_unit), or the CTA whose share the unit begins in.
 template <bool BF16>
-__device__ __forceinline__ void join_parts(const PagedParams& p, int i, int r, bool by_unit, int d, int unit_rows, RowPart* s_part) {
+__device__ __forceinline__ void join_parts(const PagedParams& p, int grid, int i, int r, bool by_unit, int d, int unit_rows, RowPart* s_part) {
   int c = i;
   int4 unit;  // parts, sequence, kv head, row tile
   if (by_unit) {
@@ -716,7 +716,7 @@ __device__ __forceinline__ void join_parts(const PagedParams& p, int i, int r, b
     unit = p.shared[c];
   }
   const int n_parts = unit.x, row = unit.w * unit_rows + r;
-  if (n_parts == 0 || row >= p.rows) return;
+  if (!parts_there(c, n_parts, grid) || row >= p.rows) return;
   const int64_t slot = static_cast<int64_t>(unit_rows) * (d + 2);
   const int columns = d / 4, groups = kTailThreads / columns, group = threadIdx.x / columns, col = (threadIdx.x - group * columns) * 4;
   const int per = (n_parts + groups - 1) / groups, end = min(n_parts, (group + 1) * per);
@@ -765,7 +765,7 @@ __device__ __forceinline__ void add_weights(const PagedParams& p, int grid, int 
     const int rt = r / unit_rows, in = r - rt * unit_rows;
     const int2 parts = p.units[static_cast<int64_t>(unit) * p.row_tiles + rt];
     float2 stat;
-    if (parts.y <= 0 || parts.x < 0 || parts.y > grid - parts.x) {  // whole (or, of lengths that changed meanwhile, nothing that is known)
+    if (!parts_there(parts.x, parts.y, grid)) {  // whole (or, of lengths that changed meanwhile, nothing that is known)
       stat = __ldcg(p.stats + static_cast<int64_t>(unit) * p.rows + r);
     } else {
       float top = -INFINITY, total = 0.f;
@@ -816,7 +816,7 @@ __global__ void __launch_bounds__(kTailThreads) paged_tail_kernel(const __grid_c
   early_trigger();
   const int i = blockIdx.x;
   if (i < joins) {
-    join_parts<BF16>(p, i % listed, i / listed, listed != grid, d, unit_rows, s.part);
+    join_parts<BF16>(p, grid, i % listed, i / listed, listed != grid, d, unit_rows, s.part);
   } else {
     const int unit = (i - joins) / blocks;
     add_weights(p, grid, unit, i - joins - unit * blocks, blocks, d, unit_rows, s.stats);

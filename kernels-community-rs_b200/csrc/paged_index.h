@@ -84,6 +84,10 @@ FA2_BOTH int share_owner(int64_t tile, int64_t tiles, int64_t grid) {
   return static_cast<int>(((tile + 1) * grid + tiles - 1) / tiles - 1);
 }
 
+// Are the parts of CTAs [first, first + n) parts of a call with `grid` CTAs? What the attention has left in the workspace says so of
+// every unit, unless the lengths were written to while it ran.
+FA2_BOTH bool parts_there(int first, int n, int grid) { return first >= 0 && n > 0 && n <= grid - first; }
+
 // Which axis turns pair i. In sections: the first sections[0] pairs belong to axis 0, and so on. In turns: of `axes` neighbours
 // each axis has one, until its section is used up; what is left belongs to axis 0.
 constexpr int kMaxAxes = 4;

@@ -311,3 +311,36 @@ def test_barriers_and_abort_words_are_seen_by_all_warps_before_their_first_wait(
         barrier = re.search(r"^  __syncthreads\(\);", body, flags=re.M)
         assert barrier is not None, (path, name)
         assert not re.search(r"(warp|mbar)_wait", body[:barrier.start()]), (path, name)
+
+
+LIST_SHIM = r'''
+#include <cuda_runtime.h>
+#include "paged_index.h"
+extern "C" int there(int first, int n, int grid) { return fa2::parts_there(first, n, grid); }
+'''
+
+
+def _library(tmp_path, source):
+    (tmp_path / "shim.cc").write_text(source)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-fsanitize=signed-integer-overflow", "-fsanitize-undefined-trap-on-error", "-shared", "-fPIC",
+                    f"-I{ROOT / 'kernels-community-rs_b200' / 'csrc'}", "-I/usr/local/cuda/include", str(tmp_path / "shim.cc"), "-o",
+                    str(tmp_path / "shim.so")], check=True)
+    return C.CDLL(str(tmp_path / "shim.so"))
+
+
+def test_parts_outside_the_workspace_are_none(tmp_path):
+    """The join reads the slots of CTAs [first, first + n): whatever the workspace says, those that there are."""
+    lib = _library(tmp_path, LIST_SHIM)
+    words = (-2 ** 31, -2 ** 31 + 1, -1, 0, 1, 2, 146, 147, 148, 149, 2 ** 30, 2 ** 31 - 148, 2 ** 31 - 1)
+    for grid in (1, 2, 148):
+        for first in words:
+            for n in words:
+                assert bool(lib.there(first, n, grid)) == (0 <= first and n > 0 and first + n <= grid), (first, n, grid)
+
+
+def test_the_join_and_the_weights_ask_for_the_parts_they_read():
+    source = (ROOT / "kernels-community-rs_b200" / "csrc" / "fwd_paged_sm100.cu").read_text()
+    for function in ("join_parts", "add_weights"):
+        body = source[source.index(f" void {function}("):]
+        body = body[:body.index("\n}\n")]
+        assert -1 < body.find("parts_there(") < body.index("part_of("), function
