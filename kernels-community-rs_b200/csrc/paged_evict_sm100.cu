@@ -285,7 +285,8 @@ __global__ void __launch_bounds__(kSelectThreads, 1) evict_select_kernel(const _
     for (int e = 0; e < 4; ++e)
       if (i + e < end) {
         const bool larger = k[e] > prefix, tie = k[e] == prefix;
-        if (larger || (tie && at_ties < ties)) kept[at_above + min(at_ties, ties)] = i + e;
+        const int place = list_place(at_above, at_ties, ties, wanted);
+        if (place >= 0 && (larger || (tie && at_ties < ties))) kept[place] = i + e;
         at_above += larger;
         at_ties += tie;
       }

@@ -88,6 +88,13 @@ FA2_BOTH int share_owner(int64_t tile, int64_t tiles, int64_t grid) {
 // every unit, unless the lengths were written to while it ran.
 FA2_BOTH bool parts_there(int first, int n, int grid) { return first >= 0 && n > 0 && n <= grid - first; }
 
+// Where a kept token goes in an eviction's list: `larger` keys and `ties` equal ones lie before it, of which the first `most_ties`
+// are kept. -1: nowhere, which only weights that are written to while the eviction reads them can make of a token that is kept.
+FA2_BOTH int list_place(int larger, int ties, int most_ties, int wanted) {
+  const int at = larger + (ties < most_ties ? ties : most_ties);
+  return at < wanted ? at : -1;
+}
+
 // Which axis turns pair i. In sections: the first sections[0] pairs belong to axis 0, and so on. In turns: of `axes` neighbours
 // each axis has one, until its section is used up; what is left belongs to axis 0.
 constexpr int kMaxAxes = 4;

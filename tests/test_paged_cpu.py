@@ -317,6 +317,7 @@ LIST_SHIM = r'''
 #include <cuda_runtime.h>
 #include "paged_index.h"
 extern "C" int there(int first, int n, int grid) { return fa2::parts_there(first, n, grid); }
+extern "C" int place(int larger, int ties, int most_ties, int wanted) { return fa2::list_place(larger, ties, most_ties, wanted); }
 '''
 
 
@@ -344,3 +345,34 @@ def test_the_join_and_the_weights_ask_for_the_parts_they_read():
         body = source[source.index(f" void {function}("):]
         body = body[:body.index("\n}\n")]
         assert -1 < body.find("parts_there(") < body.index("part_of("), function
+
+
+def test_lists_of_kept_tokens_end_where_they_should(tmp_path):
+    """The places of an eviction's list are those below `wanted`, each once, also where the weights that are counted last are not those
+    that the border was found with (more keys above it than there were)."""
+    place = _library(tmp_path, LIST_SHIM).place
+    rng = random.Random(3)
+    for _ in range(200):
+        keys = [rng.randrange(6) for _ in range(rng.randrange(2, 60))]
+        wanted = rng.randrange(1, len(keys))
+        border = sorted(keys, reverse=True)[wanted - 1]
+        ties = wanted - sum(k > border for k in keys)
+        for seen in (keys, [k + rng.randrange(3) for k in keys], [9] * len(keys)):  # as they were, and grown meanwhile
+            at_above = at_ties = 0
+            places = []
+            for k in seen:
+                at = place(at_above, at_ties, ties, wanted)
+                assert -1 <= at < wanted
+                if at >= 0 and (k > border or (k == border and at_ties < ties)):
+                    places.append(at)
+                at_above += k > border
+                at_ties += k == border
+            assert len(set(places)) == len(places)
+            if seen is keys:
+                assert places == list(range(wanted))
+
+
+def test_the_list_is_written_at_such_places():
+    source = (ROOT / "kernels-community-rs_b200" / "csrc" / "paged_evict_sm100.cu").read_text()
+    choice = source[source.index("done_above = 0"):source.index("kMoveThreads")]
+    assert "kept[place] = " in choice and choice.count("kept[") == 1 and "place = list_place(" in choice
