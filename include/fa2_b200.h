@@ -250,7 +250,9 @@ typedef struct fa2_paged_cache {
  * pairs: elements i and i + n of n pairs, or with interleaved_pairs elements 2 i and 2 i + 1; the rest is copied. A pair is
  * turned by position[axis] * inv_freq[pair], worked out so that it is exact to a few 1e-7 rad at any position below 2^31.
  * Which axis: the first sections[0] pairs have axis 0, the next sections[1] axis 1 and so on; with interleaved_axes pair i has
- * axis i % axes while i < axes * sections[i % axes], and axis 0 behind that. inverse = 1 turns back: the gradient. */
+ * axis i % axes while i < axes * sections[i % axes], and axis 0 behind that. inverse = 1 turns back: the gradient.
+ * In place: q_out may be q and k_out may be k, with the same strides. Otherwise nothing that is written may overlap anything that is
+ * read, and no two rows of an output each other. */
 typedef struct fa2_rotary_args {
   int64_t size; /* sizeof(fa2_rotary_args) */
   const void* q; /* [batch, seqlen, heads, head_dim], or NULL */

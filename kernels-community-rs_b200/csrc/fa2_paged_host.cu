@@ -36,6 +36,12 @@ bool aligned4(std::initializer_list<const void*> pointers) {
   return true;
 }
 
+// A tensor [batch, rows, heads, .] that is turned in place has to stay where it is.
+bool apart_or_in_place(const void* in, const int64_t* in_stride, const void* out, const int64_t* out_stride, int batch, int rows, int heads) {
+  if (in != out) return true;
+  return (batch <= 1 || in_stride[0] == out_stride[0]) && (rows <= 1 || in_stride[1] == out_stride[1]) && (heads <= 1 || in_stride[2] == out_stride[2]);
+}
+
 int check_types(int dtype, int head_dim) {
   if (dtype != FA2_F16 && dtype != FA2_BF16) return fail(FA2_E_TYPE, "tensors must be float16 or bfloat16");
   if (head_dim < 8 || head_dim > 256 || head_dim % 8 != 0)
@@ -109,6 +115,8 @@ int rotary_params(const fa2_rotary_args* a, fa2::RotaryParams* p) {
   if (a->q != nullptr && a->q_out == nullptr) return fail(FA2_E_VALUE, "q_out is null");
   for (const void* t : {a->q, static_cast<const void*>(a->q_out), a->k})
     if (reinterpret_cast<uintptr_t>(t) % 2) return fail(FA2_E_VALUE, "tensors must be aligned to their elements");
+  if (a->q != nullptr && !apart_or_in_place(a->q, a->q_stride, a->q_out, a->q_out_stride, a->batch, a->seqlen, a->heads))
+    return fail(FA2_E_VALUE, "q_out is q, but its strides are others");
   p->q = a->q;
   p->q_out = a->q_out;
   p->k = a->k;
@@ -206,6 +214,8 @@ int fa2_rotary(const fa2_rotary_args* args, void* stream) {
   if (p.tokens == 0 || p.heads + p.heads_k == 0) return FA2_OK;
   if (p.k != nullptr && (p.k_out == nullptr || reinterpret_cast<uintptr_t>(p.k_out) % 2))
     return fail(FA2_E_VALUE, "k_out must be non-null and aligned to its elements");
+  if (p.k != nullptr && !apart_or_in_place(p.k, args->k_stride, p.k_out, args->k_out_stride, args->batch, args->seqlen, args->heads_k))
+    return fail(FA2_E_VALUE, "k_out is k, but its strides are others");
   const DeviceScope scope(p.q != nullptr ? p.q : p.k);
   Runtime* rt = nullptr;
   if ((rc = get_runtime(scope.device(), &rt)) != FA2_OK) return rc;

@@ -201,7 +201,8 @@ __global__ void __launch_bounds__(kThreads, 8) rotary_kernel(const __grid_consta
   }
 }
 
-// Any strides and any number of pairs, two bytes at a time: a block a token.
+// Any strides and any number of pairs, two bytes at a time: a block a token. A thread reads both elements of a pair before it writes
+// either, so that the result may lie where the input was.
 template <bool BF16, bool APPEND>
 __global__ void __launch_bounds__(kThreads) rotary_any_kernel(const __grid_constant__ RotaryParams p) {
   __shared__ float2 s_turn[128];
@@ -214,23 +215,26 @@ __global__ void __launch_bounds__(kThreads) rotary_any_kernel(const __grid_const
   if (tid == 0) s_row = APPEND ? cache_row(p, t, b, s) : make_longlong2(0, 0);
   __syncthreads();
   const longlong2 row = s_row;
-  const int heads = static_cast<int>(p.heads_all.d);
+  const int heads = static_cast<int>(p.heads_all.d), items = p.head_dim - n;  // of a head: its pairs, then the elements behind them
   auto value = [](uint16_t x) { return unpack2<BF16>(x).x; };
-  for (int i = tid; i < heads * p.head_dim; i += kThreads) {
-    const int h = i / p.head_dim, e = i - h * p.head_dim;
+  for (int i = tid; i < heads * items; i += kThreads) {
+    const int h = i / items, item = i - h * items;
     const Head r = head_of<APPEND>(p, b, s, h, row);
     if (r.out == nullptr) continue;
-    if (!r.turned || e >= 2 * n) {
-      r.out[e] = r.in[e];
+    if (item >= n) {
+      r.out[n + item] = r.in[n + item];
       continue;
     }
-    const bool second = p.neighbours ? (e & 1) : e >= n;
-    const int pair = p.neighbours ? e >> 1 : second ? e - n : e;
-    const int other = p.neighbours ? e ^ 1 : second ? e - n : e + n;
-    const float2 cs = s_turn[pair];
-    const float x = value(r.in[e]), y = value(r.in[other]);
-    const float f = second ? x * cs.x + y * cs.y : x * cs.x - y * cs.y;
-    r.out[e] = static_cast<uint16_t>(pack2<BF16>(f, 0.f));
+    const int e0 = p.neighbours ? 2 * item : item, e1 = p.neighbours ? 2 * item + 1 : n + item;
+    uint16_t x0 = r.in[e0], x1 = r.in[e1];
+    if (r.turned) {
+      const float2 cs = s_turn[item];
+      const float f0 = value(x0), f1 = value(x1);
+      x0 = static_cast<uint16_t>(pack2<BF16>(f0 * cs.x - f1 * cs.y, 0.f));
+      x1 = static_cast<uint16_t>(pack2<BF16>(f1 * cs.x + f0 * cs.y, 0.f));
+    }
+    r.out[e0] = x0;
+    r.out[e1] = x1;
   }
 }
 

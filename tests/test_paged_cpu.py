@@ -376,3 +376,16 @@ def test_the_list_is_written_at_such_places():
     source = (ROOT / "kernels-community-rs_b200" / "csrc" / "paged_evict_sm100.cu").read_text()
     choice = source[source.index("done_above = 0"):source.index("kMoveThreads")]
     assert "kept[place] = " in choice and choice.count("kept[") == 1 and "place = list_place(" in choice
+
+
+@pytest.mark.parametrize("name,dim", [("q", 0), ("q", 1), ("q", 2), ("k", 0), ("k", 1), ("k", 2)])
+def test_turns_in_place_with_other_strides_are_refused(built_libs, name, dim):
+    """In place is allowed where each element stays where it is: a stride of the output that differs would make it a race."""
+    strides = [3 * 256, 256, 64]
+    other = list(strides)
+    other[dim] += 64
+    args = dict(q_stride=strides, q_out_stride=strides, k_stride=strides, k_out_stride=strides)
+    args[name + "_out_stride"] = other
+    a = _turn(**{k: tuple(v) for k, v in args.items()})
+    setattr(a, name + "_out", getattr(a, name))
+    _refused("fa2_rotary", a, -1, f"{name}_out is {name}", None)

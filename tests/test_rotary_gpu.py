@@ -314,3 +314,27 @@ def test_a_captured_backward_beside_an_eager_graph_of_the_same_leaf():
     process goes on."""
     got = _captured("rotary", "beside")
     assert got == _captured("sin", "beside") and got[-1] == "done"
+
+
+@pytest.mark.parametrize("d,sections,pad", [(128, (16, 24, 24), 0), (128, (16, 24, 24), 3), (96, (8, 12, 12), 0), (72, (3, 4, 5, 8), 0), (248, (44, 41, 39), 0)])
+@pytest.mark.parametrize("interleaved_pairs", [False, True])
+def test_in_place(d, sections, pad, interleaved_pairs):
+    """The C entry point with q_out = q and k_out = k, on tensors that 16-byte loads can take and on others (rows at odd strides, pairs that
+    are no multiple of 8): the bits of a call with other outputs, also where a call is long enough for many warps of a token."""
+    import ctypes as C
+
+    import flash_attn2_b200 as fa2
+    from flash_attn2_b200 import _cabi
+
+    b, s, h, hk = 2, 333, 24, 3
+    q, k, positions, inv_freq = (t.cuda() for t in _inputs(8, b, s, h, hk, d, sections, torch.bfloat16))
+    q, k = (torch.nn.functional.pad(t, (0, pad))[..., :d] for t in (q, k))
+    want = fa2.rotary_axes_func(q, k, positions, inv_freq, sections, interleaved_pairs=interleaved_pairs)
+    a = _cabi.RotaryArgs(size=C.sizeof(_cabi.RotaryArgs), q=q.data_ptr(), q_out=q.data_ptr(), k=k.data_ptr(), k_out=k.data_ptr(), q_stride=q.stride()[:3],
+                         q_out_stride=q.stride()[:3], k_stride=k.stride()[:3], k_out_stride=k.stride()[:3], positions=positions.data_ptr(),
+                         position_stride=positions.stride(), inv_freq=inv_freq.data_ptr(), position_bits=64, dtype=_cabi.FA2_BF16, batch=b, seqlen=s,
+                         heads=h, heads_k=hk, head_dim=d, axes=len(sections), sections=tuple(sections) + (0,) * (4 - len(sections)),
+                         interleaved_pairs=interleaved_pairs)
+    assert positions.dtype == torch.int64
+    _cabi.check(_cabi.load().fa2_rotary(C.byref(a), torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
