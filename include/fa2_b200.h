@@ -238,7 +238,9 @@ typedef struct fa2_paged_cache {
   void* k;
   void* v;
   int64_t k_stride[3], v_stride[3];
-  float* attn_mass;           /* contiguous fp32 [num_pages, heads_k, page_size], or NULL: weight that each key has got */
+  float* attn_mass;           /* contiguous fp32 [num_pages, heads_k, page_size], or NULL: weight that each key has got. The append
+                               * starts it at 0, the attention adds to it, the eviction moves it with the key; entries of rows that
+                               * hold no token may be anything */
   const int32_t* block_table; /* device int32 [batch, max_pages], unit stride in a row; entries that no token needs are ignored */
   int64_t block_table_stride;
   const int32_t* seqlens_k;   /* device int32 [batch]: tokens in the cache */
@@ -276,7 +278,8 @@ FA2_API int fa2_rotary(const fa2_rotary_args* args, void* stream);
 /* New tokens: turn->q is turned into turn->q_out, turn->k into the cache behind the seqlens_k tokens that each sequence has
  * there, and v is copied beside it; seqlens_k stays as it is. Dense: row i of sequence b is its new token i, and with
  * seqlens_new only the first seqlens_new[b] rows are. Packed (cu_seqlens; turn->batch is 1): the new tokens of sequence b are
- * the rows [cu_seqlens[b], cu_seqlens[b + 1]). Other rows are not written to the cache; every row of q is turned. */
+ * the rows [cu_seqlens[b], cu_seqlens[b + 1]). Other rows are not written to the cache; every row of q is turned. With
+ * cache->attn_mass the new tokens' entries are set to 0: a row of the pool may hold the weight of a token that lay there before. */
 typedef struct fa2_paged_append_args {
   int64_t size; /* sizeof(fa2_paged_append_args) */
   const fa2_rotary_args* turn;

@@ -257,6 +257,7 @@ int fa2_paged_append(const fa2_paged_append_args* args, void* stream) {
   p.cu_seqlens = args->cu_seqlens;
   p.seqlens_new = args->seqlens_new;
   p.sequences = c->batch;
+  p.mass = c->attn_mass;
   const bool vectors = p.pairs % 8 == 0 && addressable(p.k, t->k_stride) && addressable(p.v, args->v_stride) &&
                        (p.q == nullptr || (addressable(p.q, t->q_stride) && addressable(p.q_out, t->q_out_stride)));
   return rotary_launch(&p, t->dtype, true, vectors, rt, static_cast<cudaStream_t>(stream));

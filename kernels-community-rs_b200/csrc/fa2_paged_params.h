@@ -40,6 +40,7 @@ struct RotaryParams {
   const int32_t* cu_seqlens;    // packed: the tokens of sequence b are [cu[b], cu[b + 1])
   const int32_t* seqlens_new;   // dense: only the first of each sequence's rows are tokens
   int sequences;
+  float* mass;                  // [pages, heads_k, page_size]: a new token's weights start at 0; or null
   int* status;
 };
 

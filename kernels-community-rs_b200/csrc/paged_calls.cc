@@ -282,12 +282,12 @@ void check_written(const Tensor& t, const char* name, const char* op) {
 }
 
 Tensor append(Tensor q, Tensor k, Tensor v, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table, const Tensor& seqlens, Tensor positions,
-              Tensor inv_freq, const Turn& turn, const Tensor& cu_seqlens, const Tensor& seqlens_new) {
+              Tensor inv_freq, const Turn& turn, const Tensor& cu_seqlens, const Tensor& seqlens_new, const Tensor& mass) {
   const char* op = "paged_append";
-  refuse_transforms(op, {&q, &k, &v, &k_cache, &v_cache});
-  refuse_gradients(op, {&q, &k, &v, &k_cache, &v_cache});
+  refuse_transforms(op, {&q, &k, &v, &k_cache, &v_cache, &mass});
+  refuse_gradients(op, {&q, &k, &v, &k_cache, &v_cache, &mass});
   fa2_paged_cache c{};
-  cache_args(op, k_cache, v_cache, Tensor(), table, seqlens, c);
+  cache_args(op, k_cache, v_cache, mass, table, seqlens, c);
   check_written(k_cache, "k_cache", op);
   check_written(v_cache, "v_cache", op);
   const c10::cuda::CUDAGuard guard(k_cache.device());
@@ -323,6 +323,7 @@ Tensor append(Tensor q, Tensor k, Tensor v, const Tensor& k_cache, const Tensor&
   check(fa2_paged_append(&p, c10::cuda::getCurrentCUDAStream(guard.current_device().index()).stream()));
   written(k_cache);
   written(v_cache);
+  if (mass.defined()) written(mass);
   return q_out;
 }
 
@@ -501,20 +502,21 @@ PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 // append(q, k, v, k_cache, v_cache, block_table, seqlens_k, positions, inv_freq, sections, interleaved_axes, interleaved_pairs,
-// cu_seqlens, seqlens_new) -> q_out
+// cu_seqlens, seqlens_new, attn_mass) -> q_out
 PyObject* py_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  count(n, 14);
+  count(n, 15);
   const Tensor q = tensor_arg(args[0], "q", true), k = tensor_arg(args[1], "k"), v = tensor_arg(args[2], "v");
   const Tensor k_cache = tensor_arg(args[3], "k_cache"), v_cache = tensor_arg(args[4], "v_cache");
   const Tensor table = tensor_arg(args[5], "block_table"), seqlens = tensor_arg(args[6], "seqlens_k");
   const Tensor positions = tensor_arg(args[7], "positions"), inv_freq = tensor_arg(args[8], "inv_freq");
   const Turn turn = turn_arg(args + 9);
   const Tensor cu = tensor_arg(args[12], "cu_seqlens", true), fresh = tensor_arg(args[13], "seqlens_new", true);
+  const Tensor mass = tensor_arg(args[14], "attn_mass", true);
   Tensor out;
   {
     const WithoutPython unlocked;
-    out = append(q, k, v, k_cache, v_cache, table, seqlens, positions, inv_freq, turn, cu, fresh);
+    out = append(q, k, v, k_cache, v_cache, table, seqlens, positions, inv_freq, turn, cu, fresh, mass);
   }
   return object(out);
   END_HANDLE_TH_ERRORS

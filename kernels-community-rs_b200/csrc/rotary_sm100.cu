@@ -42,8 +42,9 @@ __device__ __forceinline__ float2 turn_of_pair(const RotaryParams& p, int b, int
   return cs;
 }
 
-// Where a new token goes: element offsets of its row (head 0) in the pools, or -1 where it is not written.
-__device__ __forceinline__ longlong2 cache_row(const RotaryParams& p, int token, int b, int s) {
+// Where a new token goes: element offsets of its row (head 0) in the pools, or -1 where it is not written. The weights that lie there
+// are those of the row's last token: this one's start at 0, for the heads first_head, first_head + 32 and so on.
+__device__ __forceinline__ longlong2 cache_row(const RotaryParams& p, int token, int b, int s, int first_head) {
   int sequence = b, i = s;
   if (p.cu_seqlens != nullptr) {
     // the last sequence that begins at or before the token
@@ -67,6 +68,8 @@ __device__ __forceinline__ longlong2 cache_row(const RotaryParams& p, int token,
     return make_longlong2(-1, -1);
   }
   const int row = p.table.page_size.mod(static_cast<int>(slot));
+  if (p.mass != nullptr)
+    for (int h = first_head; h < p.heads_k; h += 32) p.mass[(static_cast<int64_t>(page) * p.heads_k + h) * p.table.page_size.d + row] = 0.f;
   return make_longlong2(page * p.kos.outer + row * p.kos.row, page * p.vos.outer + row * p.vos.row);
 }
 
@@ -151,7 +154,7 @@ __global__ void __launch_bounds__(kThreads, 8) rotary_kernel(const __grid_consta
     s_turn[warp][1][i] = cs.y;
   }
   longlong2 row = make_longlong2(0, 0);
-  if constexpr (APPEND) row = cache_row(p, token, b, s);
+  if constexpr (APPEND) row = cache_row(p, token, b, s, (w & ((1 << p.warps_log) - 1)) == 0 ? lane : p.heads_k);  // one of a token's warps
   __syncwarp();
   float cs[16];  // cosines, then sines
   if (pairs) {
@@ -212,7 +215,10 @@ __global__ void __launch_bounds__(kThreads) rotary_any_kernel(const __grid_const
   early_trigger();
   const int t = blockIdx.x, b = p.seqlen.div(t), s = t - b * static_cast<int>(p.seqlen.d);
   for (int i = tid; i < n; i += kThreads) s_turn[i] = turn_of_pair(p, b, s, i);
-  if (tid == 0) s_row = APPEND ? cache_row(p, t, b, s) : make_longlong2(0, 0);
+  if (tid < 32) {
+    const longlong2 place = APPEND ? cache_row(p, t, b, s, tid) : make_longlong2(0, 0);
+    if (tid == 0) s_row = place;
+  }
   __syncthreads();
   const longlong2 row = s_row;
   const int heads = static_cast<int>(p.heads_all.d), items = p.head_dim - n;  // of a head: its pairs, then the elements behind them

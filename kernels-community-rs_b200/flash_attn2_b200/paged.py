@@ -10,7 +10,7 @@ on the device: a page that is not in the pool is neither read nor written and it
 the table has no room for is cut, and ``cabi_ops.device_status()`` is 100 or 101 from then on until it is read.
 
 A decoding step: ``q = paged_append(...)``, then ``paged_fwd`` with the lengths that count the new tokens, and now and then
-``paged_evict``. Prefill and training turn queries and keys with ``rotary_axes_func`` and attend with ``flash_attn_func`` or
+``paged_evict``; all three with the same ``attn_mass`` where tokens are to be evicted. Prefill and training turn queries and keys with ``rotary_axes_func`` and attend with ``flash_attn_func`` or
 ``flash_attn_varlen_func``.
 """
 from __future__ import annotations
@@ -48,15 +48,17 @@ def rotary_axes_func(q, k, positions, inv_freq, sections, interleaved_axes=False
 
 
 def paged_append(q, k, v, k_cache, v_cache, block_table, seqlens_k, positions, inv_freq, sections, interleaved_axes=False,
-                 interleaved_pairs=False, cu_seqlens=None, seqlens_new=None):
+                 interleaved_pairs=False, cu_seqlens=None, seqlens_new=None, attn_mass=None):
     """New tokens: returns q turned, and puts k, turned, and v into the cache behind the ``seqlens_k`` tokens that each
     sequence has there (``seqlens_k`` is not changed). One launch.
 
     Dense: q [B, S, H, D], k and v [B, S, Hk, D]; with ``seqlens_new`` (int32 [B]) only the first rows of each sequence are
     tokens. Packed: [T, H, D] and [T, Hk, D] with ``cu_seqlens`` (int32 [B + 1]). Rows that are no tokens go nowhere. ``q``
-    may be None. The other arguments are those of ``rotary_axes_func``. There is no gradient."""
+    may be None. With ``attn_mass`` (see ``paged_fwd``) the new tokens' entries are set to 0: pages are used again, and a row
+    keeps the weight of the token that lay there before. The other arguments are those of ``rotary_axes_func``. There is no
+    gradient."""
     return _native.append(q, k, v, k_cache, v_cache, block_table, seqlens_k, positions, inv_freq, sections, interleaved_axes,
-                          interleaved_pairs, cu_seqlens, seqlens_new)
+                          interleaved_pairs, cu_seqlens, seqlens_new, attn_mass)
 
 
 def paged_fwd(q, k_cache, v_cache, block_table, seqlens_k, out=None, attn_mass=None, softmax_scale=None, window_size_left=-1,
@@ -68,7 +70,8 @@ def paged_fwd(q, k_cache, v_cache, block_table, seqlens_k, out=None, attn_mass=N
     is divided evenly over the SMs whatever the lengths are; a call repeats itself bit for bit.
 
     ``attn_mass`` (float32 [pages, Hk, page_size], contiguous): each key's weights, summed over the query rows of its kv head,
-    are added to its entry. This takes scratch memory of 4 bytes for each head, query and key, counted with ``max_seqlen_k``
+    are added to its entry, which ``paged_append`` has started at 0 when it is given ``attn_mass`` too (a caller who does not
+    give it sets the entries of new tokens to 0 before the first call that adds to them). This takes scratch memory of 4 bytes for each head, query and key, counted with ``max_seqlen_k``
     where that is given (a bound on ``seqlens_k``; longer sequences are cut to it), else with all that the table has room
     for. There is no gradient."""
     return _native.fwd(q, k_cache, v_cache, block_table, seqlens_k, out, attn_mass, softmax_scale, window_size_left, softcap,

@@ -472,6 +472,59 @@ def test_append_without_a_place():
         assert torch.equal(now.view(torch.int16), before.view(torch.int16))
 
 
+@pytest.mark.parametrize("before,new,h,hk,d,page,sections", [
+    ([15, 16, 17], [1, 1, 1], 32, 8, 128, 16, (16, 24, 24)),     # few tokens: several warps have a token
+    ([0, 5, 100], [700, 3, 0], 8, 2, 128, 16, (24, 20, 20)),
+    ([3, 2], [9, 4], 40, 40, 72, 7, (3, 4, 5, 8)),               # two bytes at a time, more heads than lanes
+    ([0, 63], [2000, 1999], 2, 1, 64, 48, (32,)),
+], ids=str)
+@pytest.mark.parametrize("form", ["dense", "packed"])
+def test_append_starts_the_weights(before, new, h, hk, d, page, sections, form):
+    """Entries of the new tokens are 0 whatever lay there, all others the bits that they were; keys and values as without weights."""
+    import flash_attn2_b200 as fa2
+
+    b, s = len(before), max(new)
+    k, v, table = make_cache(23, [x + y for x, y in zip(before, new)], hk, d, page, torch.bfloat16)
+    g = torch.Generator().manual_seed(24)
+    q, kn, vn = (torch.randn(b, s, n, d, generator=g).bfloat16().cuda() for n in (h, hk, hk))
+    positions, freq = torch.randint(0, 1000, (len(sections), b, s), generator=g).cuda(), torch.rand(sum(sections), generator=g).cuda()
+    mass = torch.randn(k.shape[0], hk, page, generator=g).cuda()
+    mass[mass > 1] = math.nan
+    want, other = mass.clone(), (k.clone(), v.clone())
+    for i, n in enumerate(new):
+        slot = torch.arange(before[i], before[i] + n, device="cuda")
+        want[table[i].long()[slot // page], :, slot % page] = 0.0
+    extra = dict(seqlens_new=_table(new))
+    if form == "packed":
+        q, kn, vn = (torch.cat([t[i, :n] for i, n in enumerate(new)] + [t[0, :1]]) for t in (q, kn, vn))
+        positions = torch.cat([positions[:, i, :n] for i, n in enumerate(new)] + [positions[:, 0, :1]], 1)
+        extra = dict(cu_seqlens=_table([sum(new[:i]) for i in range(b + 1)]))
+    version = mass._version
+    out = fa2.paged_append(q, kn, vn, k, v, table, _table(before), positions, freq, sections, attn_mass=mass, **extra)
+    assert mass._version == version + 1
+    assert torch.equal(fa2.paged_append(q, kn, vn, *other, table, _table(before), positions, freq, sections, **extra), out)
+    for x, y in zip((k, v), other):
+        assert torch.equal(x.view(torch.int16), y.view(torch.int16))
+    assert torch.equal(mass.view(torch.int32), want.view(torch.int32))
+    was = mass.clone()                                           # tokens without a place have no entries
+    fa2.paged_append(q, kn, vn, k, v, table, _table([2 ** 31 - 1] * b), positions, freq, sections, attn_mass=mass, **extra)
+    assert fa2.cabi_ops.device_status() == 100 and torch.equal(mass.view(torch.int32), was.view(torch.int32))
+
+
+def test_append_refuses_weights_of_another_form():
+    import flash_attn2_b200 as fa2
+
+    k, v, table = make_cache(25, [40, 7], 2, 64, 16, torch.bfloat16)
+    new, n = torch.randn(2, 1, 2, 64, device="cuda").bfloat16(), _table([40, 7])
+    pos, freq, mass = torch.ones(1, 2, 1, dtype=torch.int32, device="cuda"), torch.rand(32, device="cuda"), torch.zeros(k.shape[0], 2, 16, device="cuda")
+    for kind, bad in ((ValueError, mass.transpose(1, 2)), (ValueError, mass[1:]), (TypeError, mass.double()), (NotImplementedError, mass.cpu()),
+                      (TypeError, 0.0), (RuntimeError, mass.clone().requires_grad_())):
+        was = k.clone()
+        with pytest.raises(kind):
+            fa2.paged_append(new, new, new, k, v, table, n, pos, freq, (32,), attn_mass=bad)
+        assert torch.equal(k.view(torch.int16), was.view(torch.int16))
+
+
 # ---------------------------------------------------------------- eviction
 def _masses(seed, pages, hk, page, kind):
     g = torch.Generator().manual_seed(seed)
@@ -723,3 +776,60 @@ def test_a_run_as_it_would_be_used():
     for _ in range(4):
         decode()
     assert n.tolist() == [68, 68] and fa2.cabi_ops.device_status() == 0
+
+
+@pytest.mark.parametrize("page", [16, 12])
+def test_pages_that_are_used_again(page):
+    """A server's life: sequences decode with account of their weights and are evicted again and again between two halves of a small pool,
+    whose rows hold keys and weights of tokens that are gone. Each token's weight is the sum of what it got itself, in 64 bits, and the
+    choice goes by it."""
+    import flash_attn2_b200 as fa2
+
+    b, h, hk, d, sections, budget, recent = 2, 4, 2, 64, (32,), 40, 8
+    g = torch.Generator().manual_seed(41)
+    freq = 1e4 ** (-torch.arange(32, dtype=torch.float32) / 32).cuda()
+    room = 80 // page + 1
+    k = torch.randn(4 * room, page, hk, d, generator=g).bfloat16().cuda()
+    v, mass = k.clone(), torch.full((4 * room, hk, page), math.nan, device="cuda")
+    pages = torch.randperm(4 * room, generator=g).int().cuda()
+    halves = [pages[: 2 * room].view(2, room).contiguous(), pages[2 * room:].view(2, room).contiguous()]
+    n, at = _table([0, 0]), 0
+    have = [[[] for _ in range(hk)] for _ in range(b)]           # [key, weight] of each head, in the cache's order
+    worst = 0.0                                                  # sums of the magnitudes of the scores' products
+    for life in range(4):
+        table = halves[life % 2]
+        for step in range(12):
+            count = [30, 17] if life == step == 0 else [3, 2] if step == 0 else [1, 1]
+            s = max(count)
+            q, kn, vn = (torch.randn(b, s, x, d, generator=g).bfloat16() for x in (h, hk, hk))
+            pos = (at + torch.arange(s).expand(1, b, s)).cuda()
+            at += s
+            qt = fa2.paged_append(q.cuda(), kn.cuda(), vn.cuda(), k, v, table, n, pos, freq, sections, seqlens_new=_table(count), attn_mass=mass)
+            kt = fa2.rotary_axes_func(None, kn.cuda(), pos, freq, sections)[1].cpu().double()
+            n = n + _table(count)
+            last = torch.stack([qt[i, c - 1: c] for i, c in enumerate(count)])
+            fa2.paged_fwd(last, k, v, table, n, attn_mass=mass, max_seqlen_k=room * page)
+            for i in range(b):
+                for x in range(hk):
+                    have[i][x] += [[kt[i, t, x], 0.0] for t in range(count[i])]
+                    keys = torch.stack([e[0] for e in have[i][x]])
+                    for head in range(x * (h // hk), (x + 1) * (h // hk)):
+                        qr = last[i, 0, head].cpu().double()
+                        worst = max(worst, (keys.abs() @ qr.abs()).max().item() * d ** -0.5)
+                        p = torch.softmax(keys @ qr * d ** -0.5, 0)
+                        for e, w in zip(have[i][x], p.tolist()):
+                            e[1] += w
+        to = halves[1 - life % 2]
+        lengths, kept = fa2.paged_evict(k, v, mass, table, n, to, budget, recent=recent)
+        for i in range(b):
+            for x in range(hk):
+                t = torch.arange(len(have[i][x]))
+                got = mass.cpu()[table.cpu()[i].long()[t // page], x, t % page]
+                # twice the scores' error (as in attend), exp2's 2^-22 and the roundings of up to 100 sums
+                torch.testing.assert_close(got.double(), torch.tensor([e[1] for e in have[i][x]], dtype=torch.float64),
+                                           rtol=2 * (d + 16) * 2.0 ** -23 * worst + 2.0 ** -22 + 100 * 2.0 ** -24, atol=0)
+                keep = choose(got, len(have[i][x]), budget, recent)
+                assert kept[i, x].tolist() == keep + [-1] * (budget - len(keep))
+                have[i][x] = [have[i][x][j] for j in keep]
+        n = lengths
+    assert fa2.cabi_ops.device_status() == 0
