@@ -64,7 +64,7 @@ struct PagedParams {
   int4* shared;                 // of the unit that begins in a CTA's share and ends in another: its parts (0: there is none), sequence, kv head, row tile
   float* scores;                // [batch, heads_k, rows, score_stride] in the log2 domain, or null
   int64_t score_stride;
-  float2* stats;                // [batch, heads_k, rows]: row maximum (log2 domain), 1 / row sum, where one CTA has the row's unit
+  float2* stats;                // [batch, heads_k, rows]: row maximum (log2 domain; fp16: less 7), 1 / row sum, where one CTA has the row's unit
   int2* units;                  // [batch, heads_k, row_tiles]: first CTA and number of its parts (0: it is whole); null where nothing asks for it
   float* mass;                  // [pages, heads_k, page_size]
   int* status;

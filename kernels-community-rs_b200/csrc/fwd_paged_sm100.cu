@@ -20,7 +20,9 @@
 //     pairs of keys that a fragment of V^T wants come from two such reads by byte permutes. P's fragments are transposed by movmatrix.
 //     (tcgen05 would multiply 128 rows at a time and hold P in another memory; 8 rows leave it nothing to win.)
 //   * P goes into P V as the sum of two 16-bit numbers, so that its rounding is 2^-16 (fp16: 2^-22) of it in place of 2^-8 (2^-11), and
-//     the output's error is its own rounding. mma.sync issues once in 16 cycles per scheduler here; up to 16 rows memory
+//     the output's error is its own rounding. fp16's subnormals end that for small P: in fp16 P is 2^7 times as large, which leaves an
+//     error of at most 2^-32 of the row's largest weight for each key (without, 2^-25: a first key with nearly all the weight took the
+//     weight of the thousands behind it, 6 % of an output made by their values). mma.sync issues once in 16 cycles per scheduler here; up to 16 rows memory
 //     hides that, with 32 rows the products bound the call (96 of them for 16 keys). A value that is not finite gives a result that is
 //     not finite, though an infinity may become a NaN by the two products.
 //   * Keys that no row sees are not read or count as zero, whatever lies there. Where some rows see a key and others do not, P's
@@ -467,13 +469,15 @@ __global__ void __launch_bounds__((Cfg<A, NT, TEAM>::kThreads), 1) fwd_paged_ker
           for (int e = 0; e < 4; ++e)
             if (8 * n + 2 * t4 + (e & 1) < my_rows) __stcg(out + (8 * n + (e & 1)) * p.score_stride + 8 * (e >> 1), s[n][e]);
       }
-      // ---- row maxima. The running ones hold until some score exceeds them by more than 8 (in the log2 domain): P is then at most 2^8,
-      // which costs neither of the two formats nor the fp32 sums any precision, and O is rarely rescaled.
+      // ---- the levels that P is relative to: the row maxima, in fp16 less 7. They hold until some score exceeds the maximum by more than
+      // 8 (in the log2 domain): P is then at most 2^8, in fp16 2^15, which costs neither of the two formats nor the fp32 sums any
+      // precision, and O is rarely rescaled. Sums and levels go together to what adds up parts, so that the 7 cancels there.
+      constexpr float kBelow = BF16 ? 0.f : 7.f;
       bool more = false;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) more = more || fmaxf(s[n][e], s[n][2 + e]) > m[n][e] + 8.f;
+        for (int e = 0; e < 2; ++e) more = more || fmaxf(s[n][e], s[n][2 + e]) > m[n][e] + (8.f + kBelow);
       if (__any_sync(0xffffffffu, more)) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -482,7 +486,7 @@ __global__ void __launch_bounds__((Cfg<A, NT, TEAM>::kThreads), 1) fwd_paged_ker
             float x = fmaxf(s[n][e], s[n][2 + e]);
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-            x = fmaxf(fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16)), m[n][e]);
+            x = fmaxf(fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16)) - kBelow, m[n][e]);
             const float f = part_scale(m[n][e], x);
             m[n][e] = x;
             l[n][e] *= f;

@@ -833,3 +833,29 @@ def test_pages_that_are_used_again(page):
                 have[i][x] = [have[i][x][j] for j in keep]
         n = lengths
     assert fa2.cabi_ops.device_status() == 0
+
+
+@pytest.mark.parametrize("sink", [12.0, 16.0, 17.5, 19.0])
+@pytest.mark.parametrize("h,d,page", [(1, 64, 16), (1, 128, 9), (12, 128, 16), (20, 128, 16), (20, 256, 16), (3, 192, 16)])
+def test_a_key_that_has_nearly_all_the_weight(h, d, page, sink):
+    """The first key's score is far above the others', whose weights (2^-17 to 2^-27) would be too small for fp16's subnormals as they
+    are, while their values, all of one sign, make the output: none of them gets lost. (160 sequences on the same pages, so that a
+    unit's keys lie in the warps of one or two CTAs.)"""
+    import flash_attn2_b200 as fa2
+
+    n, b, large = 2048, 160, 60000.0
+    pages = -(-n // page)
+    k = torch.zeros(pages, page, 1, d, dtype=torch.float16, device="cuda")
+    v = torch.full_like(k, large)
+    k[0, 0, 0, 0], v[0, 0] = sink, 1.0
+    q = torch.zeros(b, 1, h, d, dtype=torch.float16, device="cuda")
+    q[..., 0] = 1.0
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").expand(b, -1)
+    out, lse = fa2.paged_fwd(q, k, v, table, _table([n] * b), softmax_scale=1.0)
+    tail = (n - 1) * math.exp(-sink)
+    want = (1.0 + tail * large) / (1.0 + tail)
+    # Scores: one product, times log2 e, both roundings 2^-24 of at most 27.5; the differences' weights are off by 2^-17 of themselves. P's
+    # error is at most half a step of fp16's subnormals at 2^7 of the largest weight, 2^-32 of that, for each key.
+    atol = tail * large * 2.0 ** -17 + n * 2.0 ** -32 * large
+    torch.testing.assert_close(out.double(), torch.full_like(out, want, dtype=torch.float64), rtol=2.0 ** -11 * 1.001, atol=atol)
+    torch.testing.assert_close(lse.double(), torch.full_like(lse, sink + math.log1p(tail), dtype=torch.float64), rtol=2.0 ** -22, atol=2.0 ** -20)
