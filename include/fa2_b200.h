@@ -293,7 +293,8 @@ FA2_API int fa2_paged_append(const fa2_paged_append_args* args, void* stream);
 
 /* Attention of the last seqlen_q tokens of every sequence (which the cache holds already) over its pages: token i of them sees
  * the keys up to itself, with window_left >= 0 no more than window_left before it. At most 128 query rows per kv head
- * (seqlen_q * heads / heads_k). A row without keys gives O = 0 and LSE = +inf. With cache->attn_mass the weights of each key,
+ * (seqlen_q * heads / heads_k); a longer chunk of a prompt, once it is in the cache, goes in pieces, each with the seqlens_k that end
+ * at its own last token. A row without keys gives O = 0 and LSE = +inf. With cache->attn_mass the weights of each key,
  * summed over the query rows of its kv head, are added to it. The workspace is 256-byte aligned and may hold anything;
  * fa2_paged_fwd_workspace_bytes() bytes of it are needed (it grows with max_seqlen_k where there is attn_mass). A call
  * repeats itself bit for bit, attn_mass of pages that sequences share excepted. */

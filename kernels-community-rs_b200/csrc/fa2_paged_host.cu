@@ -195,8 +195,8 @@ int check_fwd(const fa2_paged_fwd_args* a) {
     return fail(FA2_E_VALUE, "num_heads (%d) must be a multiple of num_heads_k (%d)", a->heads, a->cache->heads_k);
   if (a->seqlen_q < 0) return fail(FA2_E_VALUE, "seqlen_q must not be negative");
   if (static_cast<int64_t>(a->seqlen_q) * (a->heads / a->cache->heads_k) > fa2::kPagedMaxRows)
-    return fail(FA2_E_VALUE, "at most %d query rows per kv head (seqlen_q * num_heads / num_heads_k), got %lld: longer chunks are for the dense or "
-                "packed forward", fa2::kPagedMaxRows, static_cast<long long>(a->seqlen_q) * (a->heads / a->cache->heads_k));
+    return fail(FA2_E_VALUE, "at most %d query rows per kv head (seqlen_q * num_heads / num_heads_k), got %lld: a longer chunk goes in "
+                "pieces, each with lengths up to its own last token", fa2::kPagedMaxRows, static_cast<long long>(a->seqlen_q) * (a->heads / a->cache->heads_k));
   if (!std::isfinite(a->softmax_scale)) return fail(FA2_E_VALUE, "softmax_scale must be finite");
   if (!std::isfinite(a->softcap) || a->softcap < 0.f) return fail(FA2_E_VALUE, "softcap must be finite and not negative");
   if (a->max_seqlen_k < 0) return fail(FA2_E_VALUE, "max_seqlen_k must not be negative");

@@ -66,7 +66,8 @@ def paged_fwd(q, k_cache, v_cache, block_table, seqlens_k, out=None, attn_mass=N
     """Attention of each sequence's last Sq tokens, which the cache holds already, over its pages: (out, LSE [B, H, Sq]).
 
     ``q`` [B, Sq, H, D] with at most 128 query rows per kv head (Sq * H / Hk). Token i of them sees the keys up to itself, and
-    with ``window_size_left`` >= 0 no more than that many before it. A row without keys gives 0 and an LSE of +inf. The work
+    with ``window_size_left`` >= 0 no more than that many before it. A longer chunk of a prompt, once it is in the cache, goes in
+    pieces: rows [i, j) of a chunk of S with ``seqlens_k - S + j``. A row without keys gives 0 and an LSE of +inf. The work
     is divided evenly over the SMs whatever the lengths are; a call repeats itself bit for bit.
 
     ``attn_mass`` (float32 [pages, Hk, page_size], contiguous): each key's weights, summed over the query rows of its kv head,

@@ -859,3 +859,28 @@ def test_a_key_that_has_nearly_all_the_weight(h, d, page, sink):
     atol = tail * large * 2.0 ** -17 + n * 2.0 ** -32 * large
     torch.testing.assert_close(out.double(), torch.full_like(out, want, dtype=torch.float64), rtol=2.0 ** -11 * 1.001, atol=atol)
     torch.testing.assert_close(lse.double(), torch.full_like(lse, sink + math.log1p(tail), dtype=torch.float64), rtol=2.0 ** -22, atol=2.0 ** -20)
+
+
+@pytest.mark.parametrize("window", [-1, 70])
+def test_a_chunk_of_a_prompt_in_pieces(window):
+    """More rows than a call takes are refused with the way to go: pieces of the chunk, each with the lengths that end at its last token,
+    are the rows of the chunk, and their weights its weights."""
+    import flash_attn2_b200 as fa2
+
+    lengths, s, h, hk, d, most = [700, 301], 301, 8, 2, 64, 32
+    k, v, table = make_cache(42, lengths, hk, d, 16, torch.bfloat16)
+    q = torch.randn(2, s, h, d, generator=torch.Generator().manual_seed(43)).bfloat16().cuda()
+    with pytest.raises(ValueError, match="in pieces, each with lengths up to its own last token"):
+        fa2.paged_fwd(q, k, v, table, _table(lengths))
+    mass = torch.zeros(k.shape[0], hk, 16, device="cuda")
+    out, lse = torch.empty_like(q), torch.empty(2, h, s, device="cuda")
+    for i in range(0, s, most):
+        j = min(s, i + most)
+        out[:, i:j], lse[:, :, i:j] = fa2.paged_fwd(q[:, i:j], k, v, table, _table(lengths) - s + j, attn_mass=mass, window_size_left=window)
+    want = attend(q, k, v, table, lengths, window=window)
+    assert fa2.cabi_ops.device_status() == 0
+    _close(out, lse, want, torch.bfloat16, v, 700)
+    for b, n in enumerate(lengths):
+        got = mass[table[b].long().clamp(min=0)].transpose(1, 2).flatten(0, 1)[:n].T.cpu().double()
+        # each piece's sum, and the additions of ten of them
+        torch.testing.assert_close(got, want[2][b], rtol=10 * 2.0 ** -24, atol=2 * want[3] * s * (h // hk))
