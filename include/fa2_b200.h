@@ -278,7 +278,7 @@ FA2_API int fa2_rotary(const fa2_rotary_args* args, void* stream);
 /* New tokens: turn->q is turned into turn->q_out, turn->k into the cache behind the seqlens_k tokens that each sequence has
  * there, and v is copied beside it; seqlens_k stays as it is. Dense: row i of sequence b is its new token i, and with
  * seqlens_new only the first seqlens_new[b] rows are. Packed (cu_seqlens; turn->batch is 1): the new tokens of sequence b are
- * the rows [cu_seqlens[b], cu_seqlens[b + 1]). Other rows are not written to the cache; every row of q is turned. With
+ * the rows [cu_seqlens[b], cu_seqlens[b + 1]). The new tokens lie outside the pools. Other rows are not written to the cache; every row of q is turned. With
  * cache->attn_mass the new tokens' entries are set to 0: a row of the pool may hold the weight of a token that lay there before. */
 typedef struct fa2_paged_append_args {
   int64_t size; /* sizeof(fa2_paged_append_args) */

@@ -297,6 +297,13 @@ Tensor append(Tensor q, Tensor k, Tensor v, const Tensor& k_cache, const Tensor&
   VALUE_CHECK(v.sizes() == k.sizes(), op, ": v must have k's shape, got ", k.sizes(), " and ", v.sizes());
   fa2_rotary_args a{};
   Tensor q_out;
+  // Tokens that lie in the pools themselves: a row may be written before it has been read.
+  for (Tensor* t : {&q, &k, &v})
+    for (const Tensor* pool : {&k_cache, &v_cache})
+      if (t->defined() && t->is_alias_of(*pool) && at::get_overlap_status(*t, *pool) != at::MemOverlapStatus::No) {
+        *t = t->clone(at::MemoryFormat::Contiguous);
+        break;
+      }
   const bool any = turn_args(op, q, k, positions, inv_freq, turn, &q_out, nullptr, a);
   v = rows(v);
   VALUE_CHECK(a.heads_k == c.heads_k && a.head_dim == c.head_dim, op, ": k must have the cache's heads and head dim, got ", k.sizes(), " and ",

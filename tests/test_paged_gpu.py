@@ -511,6 +511,23 @@ def test_append_starts_the_weights(before, new, h, hk, d, page, sections, form):
     assert fa2.cabi_ops.device_status() == 100 and torch.equal(mass.view(torch.int32), was.view(torch.int32))
 
 
+@pytest.mark.parametrize("d,sections", [(128, (64,)), (72, (20,))])
+def test_tokens_that_lie_in_the_cache(d, sections):
+    """Rows of the cache itself are appended, one place further on and over each other: all are read before any is written."""
+    import flash_attn2_b200 as fa2
+
+    n, page = 3000, 3100
+    k, v, table = make_cache(26, [page], 2, d, page, torch.bfloat16)
+    home = table[0, 0].item()
+    was = k.clone(), v.clone()
+    pos, freq = torch.zeros(1, 1, n, dtype=torch.int32, device="cuda"), torch.rand(sum(sections), device="cuda")
+    q = fa2.paged_append(k[home:home + 1, :n], k[home:home + 1, :n], v[home:home + 1, :n], k, v, table, _table([1]), pos, freq, sections)
+    assert fa2.cabi_ops.device_status() == 0 and torch.equal(q[0], was[0][home, :n])
+    for now, before in ((k, was[0]), (v, was[1])):               # at position 0 a key stays what it is
+        assert torch.equal(now[home, 1:n + 1], before[home, :n])
+        assert torch.equal(now[home, n + 1:], before[home, n + 1:]) and torch.equal(now[home, 0], before[home, 0])
+
+
 def test_append_refuses_weights_of_another_form():
     import flash_attn2_b200 as fa2
 
