@@ -389,3 +389,27 @@ def test_turns_in_place_with_other_strides_are_refused(built_libs, name, dim):
     a = _turn(**{k: tuple(v) for k, v in args.items()})
     setattr(a, name + "_out", getattr(a, name))
     _refused("fa2_rotary", a, -1, f"{name}_out is {name}", None)
+
+
+def test_tiles_of_the_kernels_size_hold_every_key_that_a_row_sees(index):
+    """The kernel's tiles have 16 keys."""
+    for n in list(range(0, 50)) + [127, 128, 129, 1000, 4093, 4096, 131071, 2 ** 31 - 70000]:
+        for sq in (1, 2, 5, 17, 128):
+            for window in (-1, 0, 1, 15, 16, 17, 63, 500, 2 ** 31 - 70001):
+                first, count = index.first_tile(n, sq, window, 16), index.tiles(n, sq, window, 16)
+                lo = max(0, n - sq - window) if window >= 0 else 0
+                assert count >= 1 and first * 16 <= lo < first * 16 + 16
+                assert (first + count) * 16 >= n
+                assert n <= first * 16 or (first + count - 1) * 16 < n
+
+
+@pytest.mark.parametrize("grid", [1, 2, 147, 148, 253, 254, 255, 256])
+@pytest.mark.parametrize("tiles", [2 ** 24 - 2, 2 ** 24 - 1, 2 ** 24, 2 ** 24 + 1])
+def test_shares_where_the_divisions_change_their_width(index, tiles, grid):
+    """Up to 2^24 - 1 tiles and 254 CTAs the products stay below 2^32 (254 * (2^24 - 1) and what share_owner adds); beyond they have 64 bits."""
+    index.begin.restype = C.c_int64
+    bounds = [index.begin(c, tiles, grid) for c in range(grid + 1)]
+    assert bounds == [c * tiles // grid for c in range(grid + 1)]
+    for c in range(grid):
+        for x in (bounds[c], bounds[c] + 1, (bounds[c] + bounds[c + 1]) // 2, bounds[c + 1] - 1):
+            assert index.owner(x, tiles, grid) == c, (x, c)
