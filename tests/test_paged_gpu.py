@@ -901,3 +901,34 @@ def test_a_chunk_of_a_prompt_in_pieces(window):
         got = mass[table[b].long().clamp(min=0)].transpose(1, 2).flatten(0, 1)[:n].T.cpu().double()
         # each piece's sum, and the additions of ten of them
         torch.testing.assert_close(got, want[2][b], rtol=10 * 2.0 ** -24, atol=2 * want[3] * s * (h // hk))
+
+
+@pytest.mark.parametrize("d", [8, 16, 40, 56, 88, 120, 136, 168, 200, 248])
+def test_head_dims_between_the_boxes(d):
+    """Pages of whole tiles at head dims that leave the last box of 64 columns partly outside."""
+    import flash_attn2_b200 as fa2
+
+    lengths = [33, 400, 0]
+    k, v, table = make_cache(44, lengths, 2, d, 32, torch.float16)
+    q = torch.randn(3, 2, 12, d, generator=torch.Generator().manual_seed(45)).half().cuda()
+    out, lse = fa2.paged_fwd(q, k, v, table, _table(lengths))
+    assert fa2.cabi_ops.device_status() == 0
+    _close(out, lse, attend(q, k, v, table, lengths), torch.float16, v, 400)
+
+
+def test_append_of_keys_alone():
+    """No queries: keys, values and weights as with them."""
+    import flash_attn2_b200 as fa2
+
+    for d, sections in ((64, (32,)), (72, (3, 4))):
+        k, v, table = make_cache(46, [20, 9], 2, d, 16, torch.float16)
+        new = torch.randn(2, 3, 2, d, generator=torch.Generator().manual_seed(47)).half().cuda()
+        pos, freq = torch.arange(3, device="cuda").expand(len(sections), 2, 3), torch.rand(sum(sections), device="cuda")
+        want, mass = (k.clone(), v.clone()), torch.ones(k.shape[0], 2, 16, device="cuda")
+        mass_want = mass.clone()
+        fa2.paged_append(new, new, new, *want, table, _table([17, 6]), pos, freq, sections, attn_mass=mass_want)
+        assert fa2.paged_append(None, new, new, k, v, table, _table([17, 6]), pos, freq, sections, attn_mass=mass) is None
+        assert fa2.cabi_ops.device_status() == 0
+        for now, w in zip((k, v), want):
+            assert torch.equal(now.view(torch.int16), w.view(torch.int16))
+        assert torch.equal(mass, mass_want) and (mass == 0).sum() == 2 * 2 * 3
