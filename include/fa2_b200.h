@@ -232,7 +232,8 @@ FA2_API int fa2_bwd_static_status(int device);
  * multiples of 8; 16-byte aligned bases), and who has which pages. Token t of sequence b lies in row t % page_size of page
  * block_table[b][t / page_size]. Two sequences may have pages in common where nothing writes to them. Entries are checked on
  * the device: a page outside the pool is neither read nor written, its keys are seen by no row, and fa2_device_status() says
- * 100; where a length exceeds what the table has room for (or max_seqlen_k) it is cut, and the status is 101. */
+ * 100; where a length exceeds what the table has room for (or max_seqlen_k) it is cut, and the status is 101. Lengths,
+ * tables and weights are not to be written while a call reads them. */
 typedef struct fa2_paged_cache {
   int64_t size; /* sizeof(fa2_paged_cache) */
   void* k;
@@ -250,7 +251,7 @@ typedef struct fa2_paged_cache {
 
 /* Rotary positions with several axes (time, height, width, ...). The first 2 * (sections[0] + ... ) elements of a head are
  * pairs: elements i and i + n of n pairs, or with interleaved_pairs elements 2 i and 2 i + 1; the rest is copied. A pair is
- * turned by position[axis] * inv_freq[pair], worked out so that it is exact to a few 1e-7 rad at any position below 2^31.
+ * turned by position[axis] * inv_freq[pair], exact to a few 1e-7 rad at any position below 2^31 (frequencies up to 1).
  * Which axis: the first sections[0] pairs have axis 0, the next sections[1] axis 1 and so on; with interleaved_axes pair i has
  * axis i % axes while i < axes * sections[i % axes], and axis 0 behind that. inverse = 1 turns back: the gradient.
  * In place: q_out may be q and k_out may be k, with the same strides. Otherwise nothing that is written may overlap anything that is

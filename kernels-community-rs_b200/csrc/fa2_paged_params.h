@@ -91,8 +91,11 @@ constexpr int kPagedMinShare = 4;    // tiles of a CTA's share at least, where t
 // Query rows of a unit.
 inline int paged_unit_rows(int rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : 32; }
 // Are the shared units found by looking at all units (fewer than CTAs), or at what each CTA has begun? With a block for each row the
-// latter leaves most of the blocks nothing to do: 32 rows against 131072 keys of 8 heads 119.6 us a call, 116.7 by units. With up to
-// 8 rows these blocks do no harm, and calls in a row are faster for them (B1 H32/8 8192 keys 13.8 us, 14.6 by units).
+// latter leaves most of the blocks nothing to do, which costs with many rows. us a call at D128, by units and by CTAs: 16 rows
+// against 8192 keys of 8 heads 20.0 and 21.2, 32 rows 28.1 and 31.2, against 131072 116.6 and 119.4, B4 12 rows 8192 keys 34.7 and 35.2.
+// Up to 8 rows it is the other way about: 4 rows against 2048 keys of 8 heads 10.8 and 10.3, 8192 17.2 and 16.7,
+// 131072 91.3 and 89.9, B4 8192 keys 31.8 and 31.5, D64 12.8 and 12.4, D256 23.1 and 22.1; only 8 rows of a single head gain by units,
+// 11.8 and 12.1. Why was not found out.
 inline bool paged_join_by_unit(int64_t units, int grid, int rows) { return units < grid && rows > 8; }
 // Floats of a partial result: O of a unit's rows, their maxima and sums.
 inline int64_t paged_part_floats(int head_dim, int rows) { return paged_unit_rows(rows) * (static_cast<int64_t>((head_dim + 63) / 64 * 64) + 2); }

@@ -11,9 +11,9 @@
 //     does not cover alone in the workspace, and a second kernel, which waits beside the first, adds the parts up (and the keys' weights).
 //   * Each warp walks key tiles of its own and keeps a queue of two or more of them in flight, 130 to 170 KB per SM: TMA boxes of 64
 //     columns where a tile lies in one page, else copies of 16 bytes by cp.async, a row's neighbouring pieces by neighbouring lanes
-//     (131072 keys of 8 heads at D128 in pages of 100 96 us, in pages of 64 91). One bulk copy for each row, for any page size, took
-//     14 cycles a row: 18 B/clk per SM, where memory gives 29. The queue goes on over the ends of units: the next unit's copies
-//     start before the warps' parts of the last one are added up.
+//     (131072 keys of 8 heads at D128 in pages of 100, 64 and 16 90 us, of 7 91, of 1 101). One bulk copy for each row, for any page
+//     size, took 14 cycles a row: 18 B/clk per SM, where the measured copy rate is 23. The queue goes on over the ends of units: the next
+//     unit's copies start before the warps' parts of the last one are added up.
 //   * The products are transposed, S^T = K Q^T and O^T = V^T P^T, by mma.sync m16n8k16: the keys (the columns of V) are the 16, 8
 //     query rows the 8, so that 8 rows, one token's heads in most models, waste nothing. Which d a k index means is free as long as
 //     K and Q agree, and so is which column of V a row of O^T is: a lane reads 16 bytes of shared memory at a time, and the
@@ -22,15 +22,17 @@
 //   * P goes into P V as the sum of two 16-bit numbers, so that its rounding is 2^-16 (fp16: 2^-22) of it in place of 2^-8 (2^-11), and
 //     the output's error is its own rounding. fp16's subnormals end that for small P: in fp16 P is 2^7 times as large, which leaves an
 //     error of at most 2^-32 of the row's largest weight for each key (without, 2^-25: a first key with nearly all the weight took the
-//     weight of the thousands behind it, 6 % of an output made by their values). mma.sync issues once in 16 cycles per scheduler here; up to 16 rows memory
-//     hides that, with 32 rows the products bound the call (96 of them for 16 keys). A value that is not finite gives a result that is
-//     not finite, though an infinity may become a NaN by the two products.
+//     weight of the thousands behind it, 6 % of an output made by their values). mma.sync issues once in 16 cycles per
+//     scheduler here; up to 16 rows memory hides that, with 32 rows the products bound the call (96 of them for 16 keys: the tensor pipe
+//     is busy 90 % of an SM's active cycles). A value that is not finite gives a result that is not finite, though an infinity may become
+//     a NaN by the two products.
 //   * Keys that no row sees are not read or count as zero, whatever lies there. Where some rows see a key and others do not, P's
 //     zero meets its value, and a value that is not finite would make a NaN of it: such values take a path of their own.
 //
-// Measured (us a call, share of the measured copy rate): B1 H32/8 D128 8192 keys 13.9 (37 %; start of the kernel, the dependent reads of
-// length, table and keys, and the join are 8 of them), 131072 keys 91 (90 %), 262144 169 (98 %); B32 4096 keys 88 (94 %); at D64 131072
-// keys 55 (74 %), at D256 165 (98 %); 4 tokens of H64/8 against 131072 keys 117 (71 %).
+// Measured (us a call, share of the measured copy rate): B1 H32/8 D128 8192 keys 14.6 (35 %; start of the kernel, the dependent reads of
+// length, table and keys, and the join are 8 of them), 131072 keys 90 (91 %), 262144 168 (98 %); B32 4096 keys 90 (92 %); at D64 131072
+// keys 55 (75 %), at D96 92 (67 %), at D192 131 (94 %), at D256 166 (99 %). 131072 keys of 8 heads with 16 rows 91 (90 %), 24 113 (73 %),
+// 32 117 (70 %), 40 208, 64 212, 96 308, 128 426 (19 %: every 32 rows read K and V again). 300 sequences of 100 tokens, 4 rows 63 (30 %).
 #include "sm100_ptx.cuh"
 #include "fa2_launch.h"
 #include "fa2_paged_params.h"

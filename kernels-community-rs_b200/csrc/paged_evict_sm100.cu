@@ -13,7 +13,8 @@
 //     of the last one to be kept and how many of the keys equal to it are; one pass in the order of the tokens then writes the
 //     list of what is kept. It is bound by the latency of its steps, a few thousand cycles.
 //   * The move, all SMs: a row's 16-byte pieces by neighbouring threads, one of K and one of V in flight in each of 2048 threads per
-//     SM. (Two or four rows a thread, and fewer threads, are slower: B16 Hk4 16384 -> 6000 87 and 92 us a call where one took 83.)
+//     SM. (Two or four rows a thread, and fewer threads, are slower: B16 Hk4 16384 -> 6000 87 and 92 us a call where one took
+//     83, all with an earlier choice.)
 //     Sources and destinations are different pages, so that the rows can move in any order and pages shared with another
 //     sequence stay as they are.
 #include <algorithm>
@@ -357,8 +358,9 @@ cudaError_t launch_paged_evict(const EvictParams& p, int sm_count, cudaStream_t 
   const int units = p.batch * p.heads_k;
   const int64_t most = p.from.capacity();
   // Clusters where there are SMs for them and more than 8192 keys for a CTA: their barriers and the exchange take longer than that many
-  // keys. us a call of B2 Hk8 from 4096 tokens with 1 CTA 12.8, with 2 15.8; of B16 Hk4 from 16384 with 1 81.9, with 2 80.6; of B1 Hk8
-  // from 131072 with 1 226, with 8 104 (an earlier state: 226, 183, 147 and 123 with 1, 2, 4 and 8).
+  // keys. us a call of B1 Hk8 from 8192 tokens with 1 CTA 12.1, with 2 13.2; from 16384 with 1 17.5, with 2 16.5; from 32768 with 1 35.8,
+  // with 2 22.2, with 4 17.1; from 131072 with 1 129, with 4 51.6, with 8 24.4; of B8 Hk8 from 8192 with 1 20.7, with 2 22.3; of B16 Hk4
+  // from 16384 with 1 82.3, with 2 80.7. (Four for 16384 tokens of few heads would take 14.1, for more heads there are no SMs.)
   const int64_t ctas = std::min<int64_t>((most + 8191) / 8192, sm_count / units);
   cudaError_t e = ctas >= 8 ? launch_select<8>(p, stream) : ctas >= 4 ? launch_select<4>(p, stream) : ctas >= 2 ? launch_select<2>(p, stream)
                                                                                                              : launch_select<1>(p, stream);

@@ -10,7 +10,8 @@
 //
 // Angles: a position of 2^20 times a frequency of 1 in 32 bits is off by 0.03 to 0.06 rad. The frequency goes, by way of fp64,
 // into turns as a fixed-point fraction of 64 bits; times the position, modulo 2^64, that is the angle's fraction of a turn, off by
-// at most position * 2^-53 * (frequency's turns) + 2^-64 * position. What is left to round is that fraction to 24 bits.
+// at most position * (2^-52 * frequency's turns + 2^-64), the constant and the product each rounded once (and 2^-54 * position where a
+// negative frequency is brought above 0). What is left to round is that fraction to 24 bits.
 #include "sm100_ptx.cuh"
 #include "fa2_launch.h"
 #include "fa2_paged_params.h"

@@ -6,12 +6,13 @@ multiple of 8 up to 256, any outer strides that are multiples of 8 elements), an
 sequence]: token t of sequence b lies in row ``t % page_size`` of page ``block_table[b, t // page_size]``. ``seqlens_k`` (int32
 [B], on the device) counts the tokens that the cache holds. Nothing is read back to the host, so that every call can be
 captured in a CUDA graph, once a first call on the device has been made outside of one. Table entries and lengths are checked
-on the device: a page that is not in the pool is neither read nor written and its keys are seen by nobody, a length that
-the table has no room for is cut, and ``cabi_ops.device_status()`` is 100 or 101 from then on until it is read.
+on the device (and are not to be written while a call reads them): a page that is not in the pool is neither read nor written
+and its keys are seen by nobody, a length that the table has no room for is cut, and ``cabi_ops.device_status()`` is 100 or 101
+from then on until it is read.
 
 A decoding step: ``q = paged_append(...)``, then ``paged_fwd`` with the lengths that count the new tokens, and now and then
-``paged_evict``; all three with the same ``attn_mass`` where tokens are to be evicted. Prefill and training turn queries and keys with ``rotary_axes_func`` and attend with ``flash_attn_func`` or
-``flash_attn_varlen_func``.
+``paged_evict``; all three with the same ``attn_mass`` where tokens are to be evicted. Prefill and training turn queries and
+keys with ``rotary_axes_func`` and attend with ``flash_attn_func`` or ``flash_attn_varlen_func``.
 """
 from __future__ import annotations
 
@@ -43,7 +44,8 @@ def rotary_axes_func(q, k, positions, inv_freq, sections, interleaved_axes=False
     pairs each of the 1 to 4 axes has. A head's first ``2 * sum(sections)`` elements are turned, the others copied: pair i
     is the elements i and i + sum(sections), with ``interleaved_pairs`` 2 i and 2 i + 1. The first sections[0] pairs belong to
     axis 0, the next to axis 1 and so on; with ``interleaved_axes`` the axes take turns, pair i belonging to axis ``i % axes``
-    while ``i < axes * sections[i % axes]`` and to axis 0 behind that. Angles are exact to a few 1e-7 rad at any position."""
+    while ``i < axes * sections[i % axes]`` and to axis 0 behind that. Angles are exact to a few 1e-7 rad
+    at any position below 2^31 (frequencies up to 1)."""
     return _native.rotary(q, k, positions, inv_freq, sections, interleaved_axes, interleaved_pairs)
 
 
@@ -68,13 +70,14 @@ def paged_fwd(q, k_cache, v_cache, block_table, seqlens_k, out=None, attn_mass=N
     ``q`` [B, Sq, H, D] with at most 128 query rows per kv head (Sq * H / Hk). Token i of them sees the keys up to itself, and
     with ``window_size_left`` >= 0 no more than that many before it. A longer chunk of a prompt, once it is in the cache, goes in
     pieces: rows [i, j) of a chunk of S with ``seqlens_k - S + j``. A row without keys gives 0 and an LSE of +inf. The work
-    is divided evenly over the SMs whatever the lengths are; a call repeats itself bit for bit.
+    is divided evenly over the SMs whatever the lengths are; a call repeats itself bit for bit, the ``attn_mass`` of pages
+    that sequences share excepted (it is added in the order of arrival).
 
     ``attn_mass`` (float32 [pages, Hk, page_size], contiguous): each key's weights, summed over the query rows of its kv head,
     are added to its entry, which ``paged_append`` has started at 0 when it is given ``attn_mass`` too (a caller who does not
-    give it sets the entries of new tokens to 0 before the first call that adds to them). This takes scratch memory of 4 bytes for each head, query and key, counted with ``max_seqlen_k``
-    where that is given (a bound on ``seqlens_k``; longer sequences are cut to it), else with all that the table has room
-    for. There is no gradient."""
+    give it sets the entries of new tokens to 0 before the first call that adds to them). This takes scratch memory of 4 bytes for
+    each head, query and key, counted with ``max_seqlen_k`` where that is given (a bound on ``seqlens_k``; longer sequences are
+    cut to it), else with all that the table has room for. There is no gradient."""
     return _native.fwd(q, k_cache, v_cache, block_table, seqlens_k, out, attn_mass, softmax_scale, window_size_left, softcap,
                        max_seqlen_k)
 
