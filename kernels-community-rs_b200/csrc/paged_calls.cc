@@ -293,6 +293,7 @@ Tensor append(Tensor q, Tensor k, Tensor v, const Tensor& k_cache, const Tensor&
   const c10::cuda::CUDAGuard guard(k_cache.device());
   on_device(k, "k", op, &k_cache);
   on_device(v, "v", op, &k_cache);
+  if (q.defined()) on_device(q, "q", op, &k_cache);
   TYPE_CHECK(v.scalar_type() == k.scalar_type() && k.scalar_type() == k_cache.scalar_type(), op, ": k, v and the cache must share dtype");
   VALUE_CHECK(v.sizes() == k.sizes(), op, ": v must have k's shape, got ", k.sizes(), " and ", v.sizes());
   fa2_rotary_args a{};

@@ -528,6 +528,20 @@ def test_tokens_that_lie_in_the_cache(d, sections):
         assert torch.equal(now[home, n + 1:], before[home, n + 1:]) and torch.equal(now[home, 0], before[home, 0])
 
 
+def test_append_refuses_tokens_without_memory():
+    """A sparse tensor, or one on the CPU, is refused before anything asks where it lies."""
+    import flash_attn2_b200 as fa2
+
+    k, v, table = make_cache(27, [4], 2, 64, 16, torch.bfloat16)
+    new, pos, freq = torch.zeros(1, 1, 2, 64, device="cuda").bfloat16(), torch.ones(1, 1, 1, dtype=torch.int32, device="cuda"), torch.rand(32, device="cuda")
+    for kind, bad in ((ValueError, new.to_sparse()), (NotImplementedError, new.cpu())):
+        for i in range(3):
+            tokens = [new] * 3
+            tokens[i] = bad
+            with pytest.raises(kind):
+                fa2.paged_append(*tokens, k, v, table, _table([4]), pos, freq, (32,))
+
+
 def test_append_refuses_weights_of_another_form():
     import flash_attn2_b200 as fa2
 
